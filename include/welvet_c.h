@@ -236,6 +236,125 @@ WELVET_API welvet_status welvet_mha_execute_device(welvet_mha_session* s, const 
                                                    float* pre, float* post, void* stream);
 WELVET_API void welvet_mha_release(welvet_mha_session* s);
 
+/* ---- paged K/V cache for decoding (no counterpart in the reference, whose
+ * attention recomputes K and V of whole sequences in every call) ----
+ * A session holds a pool of num_pages pages of page_tokens entries (a
+ * multiple of 16) for num_kv_heads K/V heads of head_dim (up to 256), and the
+ * scratch of the attention of num_heads query heads (a multiple of
+ * num_kv_heads). dtype is the cache's type: 1 (Float32), 3 (BFloat16, rounded
+ * to nearest even) or 4 (FP8E4M3: the library's codes with one fp32 scale per
+ * entry and K/V head, amax / 240 and at least 2^-96); others: code 2. A call
+ * serves up to max_seqs sequences of up to capacity = max_pages * page_tokens
+ * entries. The caller allots pages to sequences.
+ *
+ * Every call queues kernels on `stream` (a hipStream_t; null: the session's)
+ * and returns without waiting; none allocates, so all can be captured into a
+ * graph, and all lengths and tables are read on the device when they run.
+ * Calls on one session must not overlap in time, on the device either (they
+ * share the scratch); replays of graphs captured from it count as calls. */
+typedef struct welvet_kv_session welvet_kv_session;
+/* The sequences of a call: device buffers of the caller, 4-byte aligned, pos
+ * and weight 16-byte aligned.
+ *   table    [nseq][max_pages] page ids. Ids outside [0, num_pages) are holes:
+ *            nothing is written there, and their entries are as absent.
+ *   lens     [nseq] entries held (taken as within [0, capacity])
+ *   next_pos [nseq] position of the next token; null: lens (no entry of the
+ *            sequence was ever evicted)
+ *   pos      [nseq][num_kv_heads][capacity] position of every entry; null: an
+ *            entry's position is its index
+ *   weight   [nseq][num_kv_heads][capacity] running sum of the attention
+ *            weights that every entry has received; null: not kept */
+typedef struct welvet_kv_seqs {
+  int32_t nseq;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* next_pos;
+  int32_t* pos;
+  float* weight;
+} welvet_kv_seqs;
+/* flags: WELVET_KV_TRACK allots the scratch that attend needs to keep
+ * running sums (max_seqs * num_heads * capacity floats). Other bits: code 1. */
+#define WELVET_KV_TRACK 1
+WELVET_API welvet_status welvet_kv_mount(int32_t dtype, int32_t num_pages, int32_t page_tokens,
+                                         int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                         int32_t max_seqs, int32_t max_pages, int32_t flags,
+                                         welvet_kv_session** out);
+WELVET_API void welvet_kv_release(welvet_kv_session* s);
+/* The pool's device memory: k and v [num_pages][num_kv_heads][page_tokens]
+ * [pitch] elements (elements head_dim .. pitch - 1 zero), k_scale and v_scale
+ * [num_pages][num_kv_heads][page_tokens] for E4M3, else null. Pages can be
+ * copied, saved and restored as they are. */
+typedef struct welvet_kv_buffers {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pitch;
+} welvet_kv_buffers;
+WELVET_API welvet_status welvet_kv_get_buffers(welvet_kv_session* s, welvet_kv_buffers* out);
+/* Writes K and V of up to `rows` new tokens per sequence as its entries
+ * lens[b], lens[b] + 1, ...: token i < counts[b] (null: rows) of sequence b is
+ * fp32 row b * rows + i of k and v ([num_kv_heads][head_dim]; strides in
+ * floats from row to row, 0: rows follow each other). With pos, writes the
+ * positions next_pos[b] + i; with weight, clears the new entries' sums.
+ * Entries past the capacity are dropped. lens is left as it is:
+ * welvet_kv_advance_device moves it once every layer's cache is written. */
+WELVET_API welvet_status welvet_kv_append_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                                 int32_t rows, const int32_t* counts,
+                                                 const float* k, int64_t k_stride, const float* v,
+                                                 int64_t v_stride, void* stream);
+/* Entries first[b] + i (null: 0), i < counts[b] (null: count), of every
+ * sequence as fp32 into k and v [nseq][count][num_kv_heads][head_dim]; zeros
+ * behind counts[b], outside the capacity and for holes. lens is not read. */
+WELVET_API welvet_status welvet_kv_read_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                               int32_t count, const int32_t* first,
+                                               const int32_t* counts, float* k, float* v,
+                                               void* stream);
+/* Attention of one new token per sequence over its first lens[b] + tail
+ * entries (tail: those appended and not yet counted in lens). The token's
+ * position is next_pos[b] + tail - 1. q rows [num_heads][head_dim] (q_stride
+ * floats apart, 0: following each other), out alike. scale 0: 1/sqrt(head_dim).
+ * window > 0: only entries at most window - 1 positions back. alibi: scores get
+ * -2^(-8 (j + 1) / num_heads) per position between query and entry. lse
+ * [nseq][num_heads] (or null) receives the log of the sum of e^score. Without
+ * any entry to see, out is 0 and lse -inf. With weight (needs
+ * WELVET_KV_TRACK), adds to every entry's sum its weights under the
+ * num_heads / num_kv_heads query heads of the K/V head. K, V or q that are
+ * not finite, where they are seen, give outputs that are not finite; in
+ * entries that are not seen they have no effect. */
+WELVET_API welvet_status welvet_kv_attend_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                                 int32_t tail, const float* q, int64_t q_stride,
+                                                 double scale, int32_t window, int32_t alibi,
+                                                 float* out, int64_t out_stride, float* lse,
+                                                 void* stream);
+/* Eviction, first part: for every sequence and K/V head the `budget` of its
+ * lens[b] entries to keep (budget up to the capacity): entries at positions
+ * below `sinks` and at the last `recent` positions before next_pos[b], then
+ * those with the highest running sums (a sum that is NaN counts as lowest);
+ * ties go to the lowest index. sinks + recent may not exceed budget.
+ * src [nseq][num_kv_heads][budget] receives for each entry below the budget
+ * the index of what it holds afterwards: its own where that is kept, the
+ * next one kept from behind the budget where it is not (both in index order),
+ * -1 from lens[b] on. Reads lens, next_pos, pos and weight only. */
+WELVET_API welvet_status welvet_kv_choose_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                                 int32_t budget, int32_t sinks, int32_t recent,
+                                                 int32_t* src, void* stream);
+/* Eviction, second part: entry src[..][j] moves to j wherever src is at least
+ * `budget` (and within the capacity): K, V, scales, and pos and weight where
+ * given. What lies behind the budget stays as it is, so the call can be
+ * repeated. Afterwards min(lens[b], budget) entries are valid, every page
+ * behind them can be given to other sequences, and K/V heads of one sequence
+ * hold different tokens: pass next_pos, and pos where windows, ALiBi or
+ * further eviction need positions. Pages that sequences share are not for
+ * this call: it changes them for all. */
+WELVET_API welvet_status welvet_kv_compact_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                                  int32_t budget, const int32_t* src, void* stream);
+/* lens[b] becomes min(lens[b] + c, cap) and next_pos[b] (if given) grows by
+ * c = min(counts[b], add) (counts null: add). cap 0: the capacity. add 0 with
+ * cap = budget is the length after an eviction. */
+WELVET_API welvet_status welvet_kv_advance_device(welvet_kv_session* s, int32_t nseq, int32_t* lens,
+                                                  int32_t* next_pos, const int32_t* counts,
+                                                  int32_t add, int32_t cap, void* stream);
 /* Model mount with a scale scheme: schemes 1-3 re-quantize each child's fp32
  * weights (the descriptor's Dense/SwiGLU/MHA W) with that scheme; 0 is
  * welvet_model_mount. */

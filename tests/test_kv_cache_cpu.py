@@ -1,0 +1,133 @@
+"""K/V cache rules that need no GPU: refusals before a device is touched, and
+the index rules built for the host (lengths, holes in a page table, rows past
+4 GiB, E4M3 scales, the order of running sums)."""
+import ctypes
+import os
+import subprocess
+import tempfile
+
+import numpy as np
+import pytest
+
+import kv_model
+import pywelvet as pw
+
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+
+
+@pytest.fixture(scope="module")
+def rules():
+    out = os.path.join(tempfile.mkdtemp(prefix="kv_rules"), "kv.so")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC",
+                           "-I" + os.path.join(ROOT, "welvet.cuda_amd", "csrc"),
+                           os.path.join(ROOT, "tests", "host", "kv_check.cpp"), "-o", out])
+    L = ctypes.CDLL(out)
+    L.kv_check_row.restype = ctypes.c_longlong
+    L.kv_check_scale.restype = ctypes.c_float
+    L.kv_check_scale.argtypes = [ctypes.c_float]
+    L.kv_check_key.restype = ctypes.c_uint
+    L.kv_check_key.argtypes = [ctypes.c_float]
+    return L
+
+
+def mount(dtype=3, pages=4, page=16, heads=4, kv=2, hd=64, seqs=2, max_pages=2, flags=0):
+    h = ctypes.c_void_p()
+    st = pw.lib().welvet_kv_mount(dtype, pages, page, heads, kv, hd, seqs, max_pages, flags,
+                                  ctypes.byref(h))
+    return st, h
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(pages=0), 1), (dict(page=0), 1), (dict(page=17), 1), (dict(page=8), 1),
+    (dict(heads=0), 1), (dict(kv=0), 1), (dict(heads=5), 1), (dict(hd=0), 1), (dict(hd=-4), 1),
+    (dict(hd=257), 2), (dict(seqs=0), 1), (dict(seqs=65536), 1), (dict(max_pages=0), 1),
+    (dict(max_pages=1 << 27), 1), (dict(max_pages=2 ** 31 - 1, page=2 ** 31 - 16), 1),
+    (dict(flags=2), 1), (dict(dtype=0), 2), (dict(dtype=2), 2), (dict(dtype=5), 2),
+    (dict(dtype=16), 2), (dict(dtype=-1), 2),
+])
+def test_mount_refusals(bad, code):
+    st, h = mount(**bad)
+    assert st.code == code and st.message.startswith(b"kv"), st.message
+    assert not h.value
+
+
+def test_mount_without_a_device_is_code_2():
+    if pw.lib().welvet_cuda_available():
+        pytest.skip("a GPU is visible here")
+    st, h = mount()
+    assert st.code == 2 and not h.value
+    assert pw.lib().welvet_kv_mount(3, 4, 16, 4, 2, 64, 2, 2, 0, None).code == 1
+
+
+def test_null_sessions_are_refused():
+    L, q = pw.lib(), pw.KVSeqs(0, 16, 16)
+    r = ctypes.byref(q)
+    assert L.welvet_kv_append_device(None, r, 1, None, 16, 0, 16, 0, None).code == 1
+    assert L.welvet_kv_read_device(None, r, 1, None, None, 16, 16, None).code == 1
+    assert L.welvet_kv_attend_device(None, r, 0, 16, 0, 0.0, 0, 0, 16, 0, None, None).code == 1
+    assert L.welvet_kv_choose_device(None, r, 1, 0, 0, 16, None).code == 1
+    assert L.welvet_kv_compact_device(None, r, 1, 16, None).code == 1
+    assert L.welvet_kv_advance_device(None, 1, 16, None, None, 1, 0, None).code == 1
+    assert L.welvet_kv_get_buffers(None, None).code == 1
+    L.welvet_kv_release(None)
+
+
+@pytest.mark.parametrize("length,tail,cap,want", [
+    (0, 0, 32, 0), (5, 0, 32, 5), (5, 1, 32, 6), (31, 1, 32, 32), (32, 1, 32, 32),
+    (40, 0, 32, 32), (-3, 0, 32, 0), (-3, 1, 32, 1), (2 ** 31 - 1, 2 ** 31 - 1, 1 << 30, 1 << 30),
+    (-2 ** 31, 7, 32, 7),
+])
+def test_entries_of_a_sequence(rules, length, tail, cap, want):
+    assert rules.kv_check_entries(length, tail, cap) == want
+
+
+def test_rows_and_holes(rules):
+    table = (ctypes.c_int * 5)(3, -1, 0, 4, 2 ** 31 - 1)
+    pages, kv, page = 4, 3, 48
+
+    def row(e, h):
+        return rules.kv_check_row(table, e, h, pages, kv, page)
+
+    assert row(0, 0) == (3 * kv) * page and row(47, 2) == (3 * kv + 2) * page + 47
+    assert row(48, 0) == -1 and row(95, 1) == -1       # a negative page
+    assert row(96, 1) == page and row(100, 1) == page + 4
+    assert row(144, 0) == -1 and row(239, 0) == -1     # the first id past the pool, and the last int
+    big = (ctypes.c_int * 1)(2 ** 31 - 2)
+    assert rules.kv_check_row(big, 15, 7, 2 ** 31 - 1, 8, 16) == ((2 ** 31 - 2) * 8 + 7) * 16 + 15
+
+
+def test_pitch_is_whole_16_byte_pieces(rules):
+    for hd in range(1, 257):
+        for dtype, n in ((1, 4), (3, 8), (4, 16)):
+            p = rules.kv_check_pitch(dtype, hd)
+            assert p % n == 0 and hd <= p < hd + n
+
+
+def test_e4m3_scales(rules):
+    f = rules.kv_check_scale
+    assert f(0.0) == 1.0 and f(240.0) == 1.0
+    assert f(1.0) == np.float32(1) / np.float32(240)
+    assert f(1e-35) == 2.0 ** -96 and f(np.float32(2.0 ** -100)) == 2.0 ** -96
+    assert np.isnan(f(float("inf"))) and np.isnan(f(float("nan")))
+
+
+def test_order_of_running_sums(rules):
+    f = rules.kv_check_key
+    w = [float("-inf"), -3.0, -1e-45, 0.0, 1e-45, 1e-3, 1.0, 3e38, float("inf")]
+    keys = [f(x) for x in w]
+    assert keys == sorted(set(keys)) and keys[-1] < 0xFFFFFFFF
+    assert f(-0.0) == f(0.0)
+    assert f(float("nan")) < keys[0]
+
+
+def test_model_choice_of_entries():
+    """The numpy model that the GPU is compared with, on cases done by hand."""
+    f = kv_model.choose
+    at = np.arange(6)
+    w = np.float32([5, 1, 4, 4, 9, 4])
+    assert f(w, at, 6, 3, 0, 0).tolist() == [0, 4, 2]
+    assert f(w, at, 6, 2, 0, 0).tolist() == [0, 4]
+    assert f(w, at, 6, 3, 0, 1).tolist() == [0, 4, 5]
+    assert f(w, at, 6, 3, 2, 0).tolist() == [0, 1, 4]
+    assert f(w, at, 6, 8, 2, 0).tolist() == [0, 1, 2, 3, 4, 5, -1, -1]
+    assert f(np.float32([1, np.nan, 1, 1]), np.arange(4), 4, 3, 0, 0).tolist() == [0, 3, 2]

@@ -13,6 +13,7 @@
 #include <string>
 
 #include "codec.h"
+#include "kvcache.h"
 #include "layers.h"
 #include "model.h"
 #include "runtime.h"
@@ -72,6 +73,11 @@ struct welvet_mha_session {
   wv::Workspace ws;
   int batch = 0, seq = 0;
   wv::DevBuf x, pre, post;
+};
+
+struct welvet_kv_session {
+  wv::Stream stream;
+  wv::KvCache cache;
 };
 
 extern "C" {
@@ -740,6 +746,165 @@ welvet_status welvet_mha_forward_f32(int32_t batch, int32_t seq, int32_t d_model
   st = welvet_mha_execute(s, x, pre, post);
   welvet_mha_release(s);
   return st;
+}
+
+// ------------------------------------------------------------ K/V cache ----
+welvet_status welvet_kv_mount(int32_t dtype, int32_t num_pages, int32_t page_tokens,
+                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                              int32_t max_seqs, int32_t max_pages, int32_t flags,
+                              welvet_kv_session** out) {
+  if (!out) return invalid("kv: null mount args");
+  *out = nullptr;
+  if (num_pages <= 0 || page_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      max_seqs <= 0 || max_pages <= 0)
+    return invalid("kv: bad dims");
+  if (flags & ~WELVET_KV_TRACK) return invalid("kv: unknown flags");
+  if (page_tokens % wv::kKvGroup != 0) return invalid("kv: page_tokens must be a multiple of 16");
+  if (num_heads % num_kv_heads != 0)
+    return invalid("kv: num_heads must be a multiple of num_kv_heads");
+  if (dtype != wv::kKvF32 && dtype != wv::kKvBF16 && dtype != wv::kKvE4M3)
+    return to_c(Status::err(wv::kUnsupported, "kv: dtype must be Float32, BFloat16 or FP8E4M3"));
+  if (head_dim > wv::kKvMaxHd)
+    return to_c(Status::err(wv::kUnsupported, "kv: head_dim above 256"));
+  if ((int64_t)max_pages * page_tokens > (1 << 30)) return invalid("kv: capacity above 2^30");
+  if (max_seqs > 65535 || num_heads > 65535) return invalid("kv: more than 65535 sequences or heads");
+  return guarded([&]() -> Status {
+    WV_TRY(wv::init_device());
+    auto s = std::make_unique<welvet_kv_session>();
+    WV_TRY(s->stream.create());
+    WV_TRY(wv::kv_build(dtype, num_pages, page_tokens, num_heads, num_kv_heads, head_dim, max_seqs,
+                        max_pages, (flags & WELVET_KV_TRACK) != 0, &s->cache, s->stream.s));
+    *out = s.release();
+    return Status::ok();
+  });
+}
+
+void welvet_kv_release(welvet_kv_session* s) { delete s; }
+
+welvet_status welvet_kv_get_buffers(welvet_kv_session* s, welvet_kv_buffers* out) {
+  if (!s || !out) return invalid("kv: null buffers args");
+  const wv::KvPool& p = s->cache.pool;
+  *out = welvet_kv_buffers{p.k, p.v, p.ks, p.vs, p.pitch};
+  return to_c(Status::ok());
+}
+
+// The sequences of a call in the kernels' form, checked against the session.
+static Status kv_seqs(const welvet_kv_session* s, const welvet_kv_seqs* q, wv::KvSeqs* out) {
+  if (!s || !q) return Status::err(wv::kInvalid, "kv: null session or sequences");
+  if (q->nseq < 0 || q->nseq > s->cache.max_seqs)
+    return Status::err(wv::kInvalid, "kv: nseq outside the mounted number of sequences");
+  if (!q->table || !q->lens) return Status::err(wv::kInvalid, "kv: null table or lens");
+  if (((uintptr_t)q->pos | (uintptr_t)q->weight) % 16 != 0)
+    return Status::err(wv::kInvalid, "kv: pos and weight must be 16-byte aligned");
+  out->nseq = q->nseq, out->table = q->table, out->lens = q->lens, out->next_pos = q->next_pos;
+  out->pos = q->pos, out->weight = q->weight;
+  return Status::ok();
+}
+
+// A row stride: 0 stands for rows that follow each other.
+static bool kv_stride(int64_t given, int64_t width, int64_t* out) {
+  *out = given == 0 ? width : given;
+  return *out >= width;
+}
+
+welvet_status welvet_kv_append_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                      int32_t rows, const int32_t* counts, const float* k,
+                                      int64_t k_stride, const float* v, int64_t v_stride,
+                                      void* stream) {
+  return guarded([&]() -> Status {
+    wv::KvSeqs q;
+    WV_TRY(kv_seqs(s, seqs, &q));
+    const wv::KvPool& p = s->cache.pool;
+    if (rows < 0 || rows > p.capacity()) return Status::err(wv::kInvalid, "kv append: bad rows");
+    if (!k || !v) return Status::err(wv::kInvalid, "kv append: null rows");
+    wv::KvRows r;
+    const int64_t width = (int64_t)p.kv_heads * p.hd;
+    if (!kv_stride(k_stride, width, &r.k_stride) || !kv_stride(v_stride, width, &r.v_stride))
+      return Status::err(wv::kInvalid, "kv append: stride shorter than a row");
+    r.rows = rows, r.counts = counts, r.k = k, r.v = v;
+    return wv::launch_kv_append(p, q, r, pick(stream, s->stream.s));
+  });
+}
+
+welvet_status welvet_kv_read_device(welvet_kv_session* s, const welvet_kv_seqs* seqs, int32_t count,
+                                    const int32_t* first, const int32_t* counts, float* k, float* v,
+                                    void* stream) {
+  return guarded([&]() -> Status {
+    wv::KvSeqs q;
+    WV_TRY(kv_seqs(s, seqs, &q));
+    if (count < 0 || count > s->cache.pool.capacity())
+      return Status::err(wv::kInvalid, "kv read: bad count");
+    if (!k || !v) return Status::err(wv::kInvalid, "kv read: null output");
+    return wv::launch_kv_read(s->cache.pool, q, count, first, counts, k, v,
+                              pick(stream, s->stream.s));
+  });
+}
+
+welvet_status welvet_kv_attend_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                      int32_t tail, const float* q, int64_t q_stride, double scale,
+                                      int32_t window, int32_t alibi, float* out,
+                                      int64_t out_stride, float* lse, void* stream) {
+  return guarded([&]() -> Status {
+    wv::KvSeqs sq;
+    WV_TRY(kv_seqs(s, seqs, &sq));
+    const wv::KvPool& p = s->cache.pool;
+    if (!q || !out) return Status::err(wv::kInvalid, "kv attend: null q or out");
+    if (tail < 0 || tail > p.capacity()) return Status::err(wv::kInvalid, "kv attend: bad tail");
+    if (window < 0) return Status::err(wv::kInvalid, "kv attend: negative window");
+    if (!(scale >= 0.0) || scale > 3.0e38) return Status::err(wv::kInvalid, "kv attend: bad scale");
+    if (sq.weight && !s->cache.track)
+      return Status::err(wv::kInvalid, "kv attend: running sums need a session mounted with WELVET_KV_TRACK");
+    wv::KvAttend a;
+    const int64_t width = (int64_t)p.heads * p.hd;
+    if (!kv_stride(q_stride, width, &a.q_stride) || !kv_stride(out_stride, width, &a.out_stride))
+      return Status::err(wv::kInvalid, "kv attend: stride shorter than a row");
+    a.q = q, a.out = out, a.lse = lse, a.tail = tail, a.window = window, a.alibi = alibi ? 1 : 0;
+    a.scale = (float)(scale == 0.0 ? 1.0 / std::sqrt((double)p.hd) : scale);
+    return wv::kv_attend(s->cache, sq, a, pick(stream, s->stream.s));
+  });
+}
+
+welvet_status welvet_kv_choose_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                      int32_t budget, int32_t sinks, int32_t recent, int32_t* src,
+                                      void* stream) {
+  return guarded([&]() -> Status {
+    wv::KvSeqs q;
+    WV_TRY(kv_seqs(s, seqs, &q));
+    if (!q.weight || !src) return Status::err(wv::kInvalid, "kv choose: null weight or src");
+    if (budget <= 0 || budget > s->cache.pool.capacity())
+      return Status::err(wv::kInvalid, "kv choose: budget outside the capacity");
+    if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+      return Status::err(wv::kInvalid, "kv choose: sinks and recent entries exceed the budget");
+    return wv::launch_kv_choose(s->cache.pool, q, budget, sinks, recent, src,
+                                pick(stream, s->stream.s));
+  });
+}
+
+welvet_status welvet_kv_compact_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
+                                       int32_t budget, const int32_t* src, void* stream) {
+  return guarded([&]() -> Status {
+    wv::KvSeqs q;
+    WV_TRY(kv_seqs(s, seqs, &q));
+    if (!src) return Status::err(wv::kInvalid, "kv compact: null src");
+    if (budget <= 0 || budget > s->cache.pool.capacity())
+      return Status::err(wv::kInvalid, "kv compact: budget outside the capacity");
+    return wv::launch_kv_compact(s->cache.pool, q, budget, src, pick(stream, s->stream.s));
+  });
+}
+
+welvet_status welvet_kv_advance_device(welvet_kv_session* s, int32_t nseq, int32_t* lens,
+                                       int32_t* next_pos, const int32_t* counts, int32_t add,
+                                       int32_t cap, void* stream) {
+  return guarded([&]() -> Status {
+    if (!s || !lens) return Status::err(wv::kInvalid, "kv advance: null session or lens");
+    if (nseq < 0 || nseq > s->cache.max_seqs)
+      return Status::err(wv::kInvalid, "kv: nseq outside the mounted number of sequences");
+    const int capacity = s->cache.pool.capacity();
+    if (add < 0 || add > capacity || cap < 0 || cap > capacity)
+      return Status::err(wv::kInvalid, "kv advance: add or cap outside the capacity");
+    return wv::launch_kv_advance(nseq, lens, next_pos, counts, add, cap ? cap : capacity,
+                                 pick(stream, s->stream.s));
+  });
 }
 
 // ---------------------------------------------------------------- model ----

@@ -36,6 +36,19 @@ class WelvetError(RuntimeError):
         super().__init__(f"welvet status {status.code}: {status.message.decode(errors='replace')}")
 
 
+class KVSeqs(ctypes.Structure):
+    """The sequences of a K/V cache call: device pointers (welvet_kv_seqs)."""
+
+    _fields_ = [("nseq", ctypes.c_int32), ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("next_pos", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p)]
+
+
+class KVBuffers(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pitch", ctypes.c_int64)]
+
+
 _LIB = None
 OUT_OF_PATH = (
     "welvet_model_train_credit", "welvet_model_train_mse", "welvet_model_sync",
@@ -128,6 +141,19 @@ def lib():
     _sig(L, "welvet_mha_execute", Status, [_vp, _fp, _fp, _fp])
     _sig(L, "welvet_mha_execute_device", Status, [_vp, _vp, _vp, _vp, _vp])
     _sig(L, "welvet_mha_release", None, [_vp])
+    seqs = ctypes.POINTER(KVSeqs)
+    _i64 = ctypes.c_int64
+    _sig(L, "welvet_kv_mount", Status, [_i32] * 9 + [ctypes.POINTER(_vp)])
+    _sig(L, "welvet_kv_release", None, [_vp])
+    _sig(L, "welvet_kv_get_buffers", Status, [_vp, ctypes.POINTER(KVBuffers)])
+    _sig(L, "welvet_kv_append_device", Status,
+         [_vp, seqs, _i32, _vp, _vp, _i64, _vp, _i64, _vp])
+    _sig(L, "welvet_kv_read_device", Status, [_vp, seqs, _i32, _vp, _vp, _vp, _vp, _vp])
+    _sig(L, "welvet_kv_attend_device", Status,
+         [_vp, seqs, _i32, _vp, _i64, _f64, _i32, _i32, _vp, _i64, _vp, _vp])
+    _sig(L, "welvet_kv_choose_device", Status, [_vp, seqs, _i32, _i32, _i32, _vp, _vp])
+    _sig(L, "welvet_kv_compact_device", Status, [_vp, seqs, _i32, _vp, _vp])
+    _sig(L, "welvet_kv_advance_device", Status, [_vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp])
     _sig(L, "welvet_model_abi_version", _i32, [])
     _sig(L, "welvet_model_mount", Status, [_u8p, _sz, ctypes.POINTER(_vp)])
     _sig(L, "welvet_model_mount_q", Status, [_u8p, _sz, _i32, ctypes.POINTER(_vp)])
@@ -563,6 +589,65 @@ class MHASession:
     def close(self):
         if self.h:
             lib().welvet_mha_release(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+KV_F32, KV_BF16, KV_E4M3 = 1, 3, 4
+KV_TRACK = 1
+
+
+class KVCache:
+    """A paged K/V cache (welvet_kv_*). Buffers are device pointers; every call
+    returns without waiting, on `stream` or the session's own."""
+
+    def __init__(self, dtype, num_pages, page_tokens, heads, kv_heads, head_dim, max_seqs,
+                 max_pages, track=True):
+        self.h = None
+        h = _vp()
+        check(lib().welvet_kv_mount(dtype, num_pages, page_tokens, heads, kv_heads, head_dim,
+                                    max_seqs, max_pages, KV_TRACK if track else 0,
+                                    ctypes.byref(h)))
+        self.h = h
+
+    def buffers(self):
+        b = KVBuffers()
+        check(lib().welvet_kv_get_buffers(self.h, ctypes.byref(b)))
+        return b
+
+    def append(self, seqs, rows, k, v, counts=None, k_stride=0, v_stride=0, stream=None):
+        check(lib().welvet_kv_append_device(self.h, ctypes.byref(seqs), rows, counts, k, k_stride,
+                                            v, v_stride, stream))
+
+    def read(self, seqs, count, k, v, first=None, counts=None, stream=None):
+        check(lib().welvet_kv_read_device(self.h, ctypes.byref(seqs), count, first, counts, k, v,
+                                          stream))
+
+    def attend(self, seqs, q, out, tail=0, scale=0.0, window=0, alibi=False, lse=None, q_stride=0,
+               out_stride=0, stream=None):
+        check(lib().welvet_kv_attend_device(self.h, ctypes.byref(seqs), tail, q, q_stride, scale,
+                                            window, 1 if alibi else 0, out, out_stride, lse,
+                                            stream))
+
+    def choose(self, seqs, budget, sinks, recent, src, stream=None):
+        check(lib().welvet_kv_choose_device(self.h, ctypes.byref(seqs), budget, sinks, recent, src,
+                                            stream))
+
+    def compact(self, seqs, budget, src, stream=None):
+        check(lib().welvet_kv_compact_device(self.h, ctypes.byref(seqs), budget, src, stream))
+
+    def advance(self, nseq, lens, next_pos=None, counts=None, add=0, cap=0, stream=None):
+        check(lib().welvet_kv_advance_device(self.h, nseq, lens, next_pos, counts, add, cap,
+                                             stream))
+
+    def close(self):
+        if self.h:
+            lib().welvet_kv_release(self.h)
             self.h = None
 
     def __del__(self):
