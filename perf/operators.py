@@ -412,9 +412,11 @@ def _binding():
 
 
 class _Raw:
-    """Device memory of the cache as torch sees it."""
+    """Device memory of the cache as torch sees it. A tensor made of this keeps
+    it, and it keeps the cache: the memory lives as long as the tensor does."""
 
-    def __init__(self, ptr, shape, typestr):
+    def __init__(self, cache, ptr, shape, typestr):
+        self.cache = cache
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": shape, "strides": None,
                                          "typestr": typestr, "version": 2}
 
@@ -423,7 +425,7 @@ def _pool_view(case, cache, ptr, pages):
     """The pool as [page][entry][kv][hd] in the cache's type (F32 and BF16)."""
     pitch = cache.buffers().pitch
     shape = (pages, case["kv"], case["page"], pitch)
-    t = torch.as_tensor(_Raw(ptr, shape, "<f4" if case["dtype"] == "f32" else "<i2"), device="cuda")
+    t = torch.as_tensor(_Raw(cache, ptr, shape, "<f4" if case["dtype"] == "f32" else "<i2"), device="cuda")
     t = t if case["dtype"] == "f32" else t.view(torch.bfloat16)
     return t[..., :case["hd"]].permute(0, 2, 1, 3)
 
