@@ -851,7 +851,7 @@ welvet_status welvet_kv_attend_device(welvet_kv_session* s, const welvet_kv_seqs
     if (!q || !out) return Status::err(wv::kInvalid, "kv attend: null q or out");
     if (tail < 0 || tail > p.capacity()) return Status::err(wv::kInvalid, "kv attend: bad tail");
     if (window < 0) return Status::err(wv::kInvalid, "kv attend: negative window");
-    if (!(scale >= 0.0) || scale > 3.0e38) return Status::err(wv::kInvalid, "kv attend: bad scale");
+    if (!(scale >= 0.0) || scale > 2.0e38) return Status::err(wv::kInvalid, "kv attend: bad scale");
     if (sq.weight && !s->cache.track)
       return Status::err(wv::kInvalid, "kv attend: running sums need a session mounted with WELVET_KV_TRACK");
     wv::KvAttend a;
@@ -859,7 +859,7 @@ welvet_status welvet_kv_attend_device(welvet_kv_session* s, const welvet_kv_seqs
     if (!kv_stride(q_stride, width, &a.q_stride) || !kv_stride(out_stride, width, &a.out_stride))
       return Status::err(wv::kInvalid, "kv attend: stride shorter than a row");
     a.q = q, a.out = out, a.lse = lse, a.tail = tail, a.window = window, a.alibi = alibi ? 1 : 0;
-    a.scale = (float)(scale == 0.0 ? 1.0 / std::sqrt((double)p.hd) : scale);
+    a.scale2 = (float)((scale == 0.0 ? 1.0 / std::sqrt((double)p.hd) : scale) * 1.4426950408889634);
     return wv::kv_attend(s->cache, sq, a, pick(stream, s->stream.s));
   });
 }

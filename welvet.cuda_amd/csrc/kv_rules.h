@@ -62,4 +62,40 @@ WV_HD uint32_t kv_weight_key(float w) {
 }
 constexpr uint32_t kKvKeyFirst = 0xFFFFFFFFu;  // sinks and recent entries
 
+// Query heads of one K/V head are taken 16 at a time.
+WV_HD int kv_chunks(int group) { return (group + 15) / 16; }
+
+// Parts that the entries of every sequence are cut into at most, so that the
+// attention's workgroups (4 waves of up to 256 registers: two per CU) fill 256
+// CUs once; a part has at least 64 entries.
+constexpr int kKvWorkgroups = 512;
+WV_HD int kv_splits(int nseq, int kv_heads, int group, int capacity) {
+  const int64_t rows = (int64_t)nseq * kv_heads * kv_chunks(group);
+  int64_t n = kKvWorkgroups / rows;
+  const int most = (capacity + 63) / 64;
+  n = n < most ? n : most;
+  return n > 1 ? (int)n : 1;
+}
+
+// A sequence's tiles of `kt` entries [first, end) and the tiles of each of its
+// `parts`. window: of positions that are indices (0: none).
+struct KvRange {
+  int first, end, step, parts;
+};
+WV_HD KvRange kv_range(int n, int qp, int window, int kt, int splits) {
+  KvRange r;
+  r.end = (n + kt - 1) / kt;
+  r.first = 0;
+  if (window > 0 && qp >= window) {
+    const int e = qp - window + 1;  // the first entry inside
+    r.first = e / kt < r.end ? e / kt : r.end;
+  }
+  const int tiles = r.end - r.first;
+  const int least = 64 / kt;
+  r.step = (tiles + splits - 1) / splits;
+  r.step = r.step < least ? least : r.step;
+  r.parts = (tiles + r.step - 1) / r.step;
+  return r;
+}
+
 }  // namespace wv

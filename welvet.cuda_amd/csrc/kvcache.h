@@ -37,7 +37,8 @@ struct KvCache {
   int max_seqs = 0;
   bool track = false;
   DevBuf k, v, ks, vs;
-  DevBuf scores;  // [max_seqs][heads][capacity]
+  DevBuf part, part_ml;  // KvPart::out and ml
+  DevBuf scores, lse2;   // track: KvPart::scores and lse2
 };
 Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_heads, int hd,
                 int max_seqs, int max_pages, bool track, KvCache* c, hipStream_t st);
@@ -60,7 +61,18 @@ struct KvAttend {
   float* lse = nullptr;      // [nseq][heads] or null
   int64_t q_stride = 0, out_stride = 0;
   int tail = 0, window = 0, alibi = 0;
-  float scale = 0.0f;
+  float scale2 = 0.0f;  // scale * log2(e)
+};
+// Scratch of an attention call. ml and out: per (sequence, head, part) the
+// reference and sum of the weights and the unscaled sums of V, used by
+// sequences of more than one part; scores (log2 units) and lse2: for the
+// running sums, null without.
+struct KvPart {
+  int splits = 1;
+  float* out = nullptr;     // [nseq][heads][splits][hd]
+  float* ml = nullptr;      // [nseq][heads][splits][2]
+  float* scores = nullptr;  // [nseq][heads][capacity]
+  float* lse2 = nullptr;    // [nseq][heads]
 };
 Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream_t st);
 
