@@ -272,8 +272,9 @@ typedef struct welvet_kv_seqs {
   int32_t* pos;
   float* weight;
 } welvet_kv_seqs;
-/* flags: WELVET_KV_TRACK allots the scratch that attend needs to keep
- * running sums (max_seqs * num_heads * capacity floats). Other bits: code 1. */
+/* flags: WELVET_KV_TRACK allots the scratch that attend needs to keep running
+ * sums (max_seqs * num_heads * capacity floats) and that choose needs. Other
+ * bits: code 1. */
 #define WELVET_KV_TRACK 1
 WELVET_API welvet_status welvet_kv_mount(int32_t dtype, int32_t num_pages, int32_t page_tokens,
                                          int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -335,7 +336,8 @@ WELVET_API welvet_status welvet_kv_attend_device(welvet_kv_session* s, const wel
  * src [nseq][num_kv_heads][budget] receives for each entry below the budget
  * the index of what it holds afterwards: its own where that is kept, the
  * next one kept from behind the budget where it is not (both in index order),
- * -1 from lens[b] on. Reads lens, next_pos, pos and weight only. */
+ * -1 from lens[b] on. Reads lens, next_pos, pos and weight only. Needs
+ * WELVET_KV_TRACK. */
 WELVET_API welvet_status welvet_kv_choose_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
                                                  int32_t budget, int32_t sinks, int32_t recent,
                                                  int32_t* src, void* stream);

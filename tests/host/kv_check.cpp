@@ -15,4 +15,18 @@ float kv_check_scale(float amax) { return wv::kv_e4m3_scale(amax); }
 
 unsigned kv_check_key(float w) { return wv::kv_weight_key(w); }
 
+int kv_check_target(int rows) { return wv::kv_target(rows); }
+
+int kv_check_part_tiles(long long tiles, int target, int kt) { return wv::kv_part_tiles(tiles, target, kt); }
+
+int kv_check_parts(int tiles, int part_tiles) { return wv::kv_parts(tiles, part_tiles); }
+
+long long kv_check_most_parts(int nseq, int target, int capacity) {
+  return wv::kv_most_parts(nseq, target, capacity);
+}
+
+long long kv_check_most_slots(int target) { return wv::kv_most_slots(target); }
+
+int kv_check_first_tile(int n, int qp, int window, int kt) { return wv::kv_first_tile(n, qp, window, kt); }
+
 }  // extern "C"

@@ -191,6 +191,22 @@ def test_attend_over_long_caches(hip, oracle, dtype, lens, heads, kv, hd):
     c.close()
 
 
+@pytest.mark.parametrize("nseq,most,heads,kv,hd,dtype", [
+    (70, 700, 2, 1, 64, km.E4M3), (130, 300, 20, 1, 32, km.BF16), (64, 900, 4, 4, 16, km.F32),
+    (65, 2000, 1, 1, 64, km.BF16), (3, 4000, 34, 2, 64, km.BF16),
+])
+def test_attend_over_many_unequal_sequences(hip, oracle, nseq, most, heads, kv, hd, dtype):
+    """Sequences of none to many parts in one call, joined by kind."""
+    rng = np.random.default_rng(nseq)
+    lens = (most * rng.random(nseq) ** 3).astype(int)
+    lens[rng.random(nseq) < 0.2] = 0
+    lens[nseq // 2] = most
+    c = filled(hip, oracle, lens.tolist(), dtype, heads, kv, hd, 16, seed=nseq)
+    check(c, query(c.rng, c))
+    check(c, query(c.rng, c), window=257)
+    c.close()
+
+
 @pytest.mark.parametrize("window,alibi,tail,scale", [
     (1, False, 0, 0.0), (17, False, 1, 0.0), (64, True, 0, 0.0), (1000, True, 1, 0.05),
     (0, True, 0, 0.0), (0, False, 1, 0.3), (2 ** 31 - 1, False, 0, 0.0), (300, False, 5, 0.0),
@@ -405,7 +421,10 @@ def weights(rng, shape, kind):
     ([1, 2, 0, 17], 1, 0, 0, False), ([33, 32, 31, 100], 32, 4, 16, False),
     ([1024, 1025, 1026, 2500], 1024, 4, 200, True), ([2100, 3000, 1, 700], 2100, 0, 2100, False),
     ([2100, 3000, 1, 700], 5, 5, 0, True), ([5000, 4999, 64, 65], 64, 0, 0, True),
-    ([4096, 4000, 2049, 2047], 2048, 1000, 1000, True),
+    ([4096, 4000, 2049, 2047], 2048, 1000, 1000, True), ([16384, 9000], 9000, 4, 100, False),
+    # (one workgroup's most entries; several segments, their edges, long and short rows together)
+    ([32768, 20001], 16384, 4, 1000, True), ([32785, 32768, 500, 40000, 1], 1, 0, 1, False),
+    ([70001, 16384, 16385, 49152], 16384, 4, 1000, True), ([70001, 60000, 34000], 33000, 40, 20000, False),
 ])
 def test_choose(hip, lens, budget, sinks, recent, positions, kind):
     page = 16
@@ -421,7 +440,8 @@ def test_choose(hip, lens, budget, sinks, recent, positions, kind):
     if positions:
         c.put(c.d_pos, c.pos)
     src = c.up(np.full((len(lens) + 1, 3, budget), 99, np.int32))
-    c.c.choose(c.seqs, budget, sinks, recent, src)
+    for _ in range(2):  # (the second call finds the scratch as it was)
+        c.c.choose(c.seqs, budget, sinks, recent, src)
     got = c.down(src, (len(lens) + 1, 3, budget), np.int32)
     for b, n in enumerate(lens):
         for h in range(3):

@@ -23,6 +23,9 @@ def rules():
                            os.path.join(ROOT, "tests", "host", "kv_check.cpp"), "-o", out])
     L = ctypes.CDLL(out)
     L.kv_check_row.restype = ctypes.c_longlong
+    for name in ("most_parts", "most_slots"):
+        getattr(L, "kv_check_" + name).restype = ctypes.c_longlong
+    L.kv_check_part_tiles.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     L.kv_check_scale.restype = ctypes.c_float
     L.kv_check_scale.argtypes = [ctypes.c_float]
     L.kv_check_key.restype = ctypes.c_uint
@@ -131,3 +134,34 @@ def test_model_choice_of_entries():
     assert f(w, at, 6, 3, 2, 0).tolist() == [0, 1, 4]
     assert f(w, at, 6, 8, 2, 0).tolist() == [0, 1, 2, 3, 4, 5, -1, -1]
     assert f(np.float32([1, np.nan, 1, 1]), np.arange(4), 4, 3, 0, 0).tolist() == [0, 3, 2]
+
+
+def test_parts_fit_the_grid_and_the_scratch(rules):
+    """The attention's cut: every tile in one part, never more parts than the
+    grid has, nor more slots than the scratch."""
+    rng = np.random.default_rng(5)
+    for _ in range(3000):
+        kt = int(rng.choice([16, 32]))
+        cap = 16 * int(np.exp(rng.uniform(0, 9)))
+        nseq, rows = int(np.exp(rng.uniform(0, 6))), int(np.exp(rng.uniform(0, 7)))
+        lens = rng.integers(0, cap + 1, nseq)
+        if rng.random() < 0.5:  # a few long ones
+            lens = np.where(rng.random(nseq) < 0.1, lens, lens // 50)
+        tiles = [-(-int(n) // kt) for n in lens]
+        target = rules.kv_check_target(rows)
+        step = rules.kv_check_part_tiles(sum(tiles), target, kt)
+        parts = [rules.kv_check_parts(t, step) for t in tiles]
+        assert all(p >= 1 and (p - 1) * step < max(t, 1) <= p * step for p, t in zip(parts, tiles))
+        assert sum(parts) <= rules.kv_check_most_parts(nseq, target, cap)
+        assert sum(p for p in parts if p > 1) < max(1, rules.kv_check_most_slots(target))
+
+
+def test_first_tile_of_a_window(rules):
+    for n in (0, 1, 31, 32, 33, 500):
+        for window in (0, 1, 5, 32, 499, 500, 2 ** 31 - 1):
+            for qp in (0, n - 1, n, n + 3, n + 600):
+                for kt in (16, 32):
+                    t = rules.kv_check_first_tile(n, qp, window, kt)
+                    seen = [e for e in range(n) if not window or qp - e < window]
+                    assert 0 <= t * kt <= n
+                    assert not seen or t * kt <= seen[0] < t * kt + kt

@@ -871,11 +871,13 @@ welvet_status welvet_kv_choose_device(welvet_kv_session* s, const welvet_kv_seqs
     wv::KvSeqs q;
     WV_TRY(kv_seqs(s, seqs, &q));
     if (!q.weight || !src) return Status::err(wv::kInvalid, "kv choose: null weight or src");
+    if (!s->cache.track)
+      return Status::err(wv::kInvalid, "kv choose: needs a session mounted with WELVET_KV_TRACK");
     if (budget <= 0 || budget > s->cache.pool.capacity())
       return Status::err(wv::kInvalid, "kv choose: budget outside the capacity");
     if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
       return Status::err(wv::kInvalid, "kv choose: sinks and recent entries exceed the budget");
-    return wv::launch_kv_choose(s->cache.pool, q, budget, sinks, recent, src,
+    return wv::kv_choose(s->cache, q, budget, sinks, recent, src,
                                 pick(stream, s->stream.s));
   });
 }

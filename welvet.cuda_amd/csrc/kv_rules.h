@@ -65,37 +65,41 @@ constexpr uint32_t kKvKeyFirst = 0xFFFFFFFFu;  // sinks and recent entries
 // Query heads of one K/V head are taken 16 at a time.
 WV_HD int kv_chunks(int group) { return (group + 15) / 16; }
 
-// Parts that the entries of every sequence are cut into at most, so that the
-// attention's workgroups (4 waves of up to 256 registers: two per CU) fill 256
-// CUs once; a part has at least 64 entries.
-constexpr int kKvWorkgroups = 512;
-WV_HD int kv_splits(int nseq, int kv_heads, int group, int capacity) {
-  const int64_t rows = (int64_t)nseq * kv_heads * kv_chunks(group);
-  int64_t n = kKvWorkgroups / rows;
-  const int most = (capacity + 63) / 64;
-  n = n < most ? n : most;
-  return n > 1 ? (int)n : 1;
+// The attention's workgroups take parts of the sequences' entries, in tiles of
+// `kt`. The parts of all sequences are alike: about `target` of them would
+// take every tile (kv_part_tiles), so that unequal sequences keep the GPU
+// evenly busy; a sequence has one at least. `target` counts the parts per K/V
+// head and chunk of its query heads.
+constexpr int kKvWorkgroups = 512;  // two per CU: 4 waves of up to 256 registers
+WV_HD int kv_target(int kv_rows) {
+  const int n = kKvWorkgroups / kv_rows;
+  return n > 1 ? n : 1;
 }
+constexpr int kKvLeastEntries = 256;  // two tiles for each of a workgroup's waves
+WV_HD int kv_part_tiles(int64_t tiles, int target, int kt) {
+  const int64_t n = (tiles + target - 1) / target;
+  return n > kKvLeastEntries / kt ? (int)n : kKvLeastEntries / kt;
+}
+WV_HD int kv_parts(int tiles, int part_tiles) {
+  const int n = (tiles + part_tiles - 1) / part_tiles;
+  return n > 1 ? n : 1;
+}
+// Most parts of all sequences: every tile in part_tiles' share, and one that
+// is not full per sequence.
+WV_HD int64_t kv_most_parts(int nseq, int target, int capacity) {
+  const int64_t by_target = (int64_t)target + nseq;
+  const int64_t by_capacity = (int64_t)nseq * ((capacity + kKvLeastEntries - 1) / kKvLeastEntries);
+  return by_target < by_capacity ? by_target : by_capacity;
+}
+// Most parts of the sequences that have more than one: their tiles exceed a
+// part each, so there are fewer than `target` of them.
+WV_HD int64_t kv_most_slots(int target) { return 2 * (int64_t)target; }
 
-// A sequence's tiles of `kt` entries [first, end) and the tiles of each of its
-// `parts`. window: of positions that are indices (0: none).
-struct KvRange {
-  int first, end, step, parts;
-};
-WV_HD KvRange kv_range(int n, int qp, int window, int kt, int splits) {
-  KvRange r;
-  r.end = (n + kt - 1) / kt;
-  r.first = 0;
-  if (window > 0 && qp >= window) {
-    const int e = qp - window + 1;  // the first entry inside
-    r.first = e / kt < r.end ? e / kt : r.end;
-  }
-  const int tiles = r.end - r.first;
-  const int least = 64 / kt;
-  r.step = (tiles + splits - 1) / splits;
-  r.step = r.step < least ? least : r.step;
-  r.parts = (tiles + r.step - 1) / r.step;
-  return r;
+// First tile of `kt` entries that a window over indices leaves (0: no window).
+WV_HD int kv_first_tile(int n, int qp, int window, int kt) {
+  if (window <= 0 || qp < window) return 0;
+  const int e = qp - window + 1;
+  return (e < n ? e : n) / kt;
 }
 
 }  // namespace wv

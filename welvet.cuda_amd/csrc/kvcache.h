@@ -37,8 +37,10 @@ struct KvCache {
   int max_seqs = 0;
   bool track = false;
   DevBuf k, v, ks, vs;
-  DevBuf part, part_ml;  // KvPart::out and ml
+  DevBuf part, part_ml, info;  // KvPart::out, ml, info
   DevBuf scores, lse2;   // track: KvPart::scores and lse2
+  // track, long capacities: the scratch of kv_choose (KvChooseLong)
+  DevBuf choose_hist, choose_cut, choose_counts, choose_list;
 };
 Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_heads, int hd,
                 int max_seqs, int max_pages, bool track, KvCache* c, hipStream_t st);
@@ -63,21 +65,23 @@ struct KvAttend {
   int tail = 0, window = 0, alibi = 0;
   float scale2 = 0.0f;  // scale * log2(e)
 };
-// Scratch of an attention call. ml and out: per (sequence, head, part) the
-// reference and sum of the weights and the unscaled sums of V, used by
-// sequences of more than one part; scores (log2 units) and lse2: for the
-// running sums, null without.
+// How an attention call is cut, and its scratch. ml and out: per slot (a part
+// of a sequence of more than one), row of query heads (K/V head and chunk of
+// 16 heads) and head the reference and sum of the weights and the unscaled
+// sums of V; info: a sequence's first slot and number of parts; scores (log2
+// units) and lse2: for the running sums, null without.
 struct KvPart {
-  int splits = 1;
-  float* out = nullptr;     // [nseq][heads][splits][hd]
-  float* ml = nullptr;      // [nseq][heads][splits][2]
-  float* scores = nullptr;  // [nseq][heads][capacity]
-  float* lse2 = nullptr;    // [nseq][heads]
+  int target = 0;             // kv_target; 0: every sequence is one part
+  float* out = nullptr;       // [slots][rows][heads of a row][hd up to 4]
+  float* ml = nullptr;        // [slots][rows][heads of a row][2]
+  int32_t* info = nullptr;    // [nseq][2], null where nothing follows the parts
+  float* scores = nullptr;    // [nseq][heads][capacity]
+  float* lse2 = nullptr;      // [nseq][heads]
 };
 Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream_t st);
 
-Status launch_kv_choose(const KvPool& p, const KvSeqs& s, int budget, int sinks, int recent,
-                        int32_t* src, hipStream_t st);
+Status kv_choose(const KvCache& c, const KvSeqs& s, int budget, int sinks, int recent, int32_t* src,
+                 hipStream_t st);
 Status launch_kv_compact(const KvPool& p, const KvSeqs& s, int budget, const int32_t* src,
                          hipStream_t st);
 Status launch_kv_advance(int nseq, int32_t* lens, int32_t* next_pos, const int32_t* counts, int add,

@@ -21,12 +21,6 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float load_elem(const uint8_t* row, int dtype, int d) {
-  if (dtype == kKvF32) return reinterpret_cast<const float*>(row)[d];
-  if (dtype == kKvBF16) return float_of((uint32_t) reinterpret_cast<const uint16_t*>(row)[d] << 16);
-  return decode_e4m3(row[d]);
-}
-
 // ---------------------------------------------------------------------------
 // Append: one group of lanes per (token, K/V head), four elements of its K
 // and V rows per lane.
@@ -81,63 +75,98 @@ __device__ __forceinline__ void store_row4(uint8_t* row, float* scale, v4f x, in
   }
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(256) void k_kv_append(KvPool p, KvSeqs s, KvRows r, int lanes,
-                                                   int64_t groups) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
-  const int d = 4 * (threadIdx.x & (lanes - 1));
-  if (i >= groups) return;
-  const int h = (int)(i % p.kv_heads);
-  const int64_t t = i / p.kv_heads;  // token row
-  const int b = (int)(t / r.rows), j = (int)(t % r.rows);
-  if (r.counts && j >= r.counts[b]) return;
-  const int cap = p.capacity();
-  const int len = s.lens[b];
-  const int e = kv_entries(len, 0, cap) + j;
+// A workgroup's groups of lanes over the rows of sequence blockIdx.y.
+struct RowPlace {
+  int b, j, h, d;  // sequence, token, K/V head, first element
+  int64_t t;       // token row: b * rows + j
+};
+__device__ __forceinline__ bool row_place(const KvPool& p, int rows, int lanes, RowPlace& r) {
+  const uint32_t i = (blockIdx.x * 256u + threadIdx.x) / (uint32_t)lanes;
+  if (i >= (uint32_t)rows * (uint32_t)p.kv_heads) return false;
+  r.b = blockIdx.y;
+  r.j = (int)(i / (uint32_t)p.kv_heads);
+  r.h = (int)(i - (uint32_t)r.j * (uint32_t)p.kv_heads);
+  r.d = 4 * (threadIdx.x & (lanes - 1));
+  r.t = (int64_t)r.b * rows + r.j;
+  return true;
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void k_kv_append(KvPool p, KvSeqs s, KvRows r, int lanes) {
+  RowPlace at;
+  if (!row_place(p, r.rows, lanes, at)) return;
+  if (r.counts && at.j >= r.counts[at.b]) return;
+  const int cap = p.capacity(), h = at.h, d = at.d;
+  const int len = s.lens[at.b];
+  const int e = kv_entries(len, 0, cap) + at.j;
   if (e >= cap) return;
-  const int64_t row = kv_row(s.table + (size_t)b * p.max_pages, e, h, p.num_pages, p.kv_heads,
+  const v4f kx = load_row4<VEC>(r.k + at.t * r.k_stride + (size_t)h * p.hd, d, p.hd);
+  const v4f vx = load_row4<VEC>(r.v + at.t * r.v_stride + (size_t)h * p.hd, d, p.hd);
+  const int64_t row = kv_row(s.table + (size_t)at.b * p.max_pages, e, h, p.num_pages, p.kv_heads,
                              p.page_tokens);
   if (d == 0) {
-    const size_t at = ((size_t)b * p.kv_heads + h) * cap + e;
-    if (s.pos) s.pos[at] = (s.next_pos ? s.next_pos[b] : len < 0 ? 0 : len) + j;
-    if (s.weight) s.weight[at] = 0.0f;
+    const size_t i = ((size_t)at.b * p.kv_heads + h) * cap + e;
+    if (s.pos) s.pos[i] = (s.next_pos ? s.next_pos[at.b] : len < 0 ? 0 : len) + at.j;
+    if (s.weight) s.weight[i] = 0.0f;
   }
   if (row < 0) return;
-  const v4f kx = load_row4<VEC>(r.k + t * r.k_stride + (size_t)h * p.hd, d, p.hd);
-  const v4f vx = load_row4<VEC>(r.v + t * r.v_stride + (size_t)h * p.hd, d, p.hd);
-  const size_t at = (size_t)row * p.pitch * kv_elem_bytes(p.dtype);
-  store_row4(p.k + at, p.ks + row, kx, p.dtype, d, p.pitch, lanes);
-  store_row4(p.v + at, p.vs + row, vx, p.dtype, d, p.pitch, lanes);
+  const size_t o = (size_t)row * p.pitch * kv_elem_bytes(DT);
+  store_row4(p.k + o, p.ks + row, kx, DT, d, p.pitch, lanes);
+  store_row4(p.v + o, p.vs + row, vx, DT, d, p.pitch, lanes);
 }
 
 // ---------------------------------------------------------------------------
 // Read: entries first[b] + i as fp32, i < counts[b]; zero behind.
+template <bool VEC>
+__device__ __forceinline__ void write_row4(float* row, v4f x, int d, int hd) {
+  if constexpr (VEC) {
+    if (d < hd) *reinterpret_cast<v4f*>(row + d) = x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (d + j < hd) row[d + j] = x[j];
+  }
+}
+
+// Elements d .. d + 3 of a row (d a multiple of 4 below the pitch).
+template <int DT>
+__device__ __forceinline__ v4f read_row4(const uint8_t* row, int d) {
+  if constexpr (DT == kKvF32) {
+    return *reinterpret_cast<const v4f*>(row + 4 * (size_t)d);
+  } else if constexpr (DT == kKvBF16) {
+    const uint2 w = *reinterpret_cast<const uint2*>(row + 2 * (size_t)d);
+    return v4f{float_of(w.x << 16), float_of(w.x & 0xFFFF0000u), float_of(w.y << 16),
+               float_of(w.y & 0xFFFF0000u)};
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + d);
+    return v4f{decode_e4m3((uint8_t)w), decode_e4m3((uint8_t)(w >> 8)),
+               decode_e4m3((uint8_t)(w >> 16)), decode_e4m3((uint8_t)(w >> 24))};
+  }
+}
+
+template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void k_kv_read(KvPool p, KvSeqs s, int count,
                                                  const int32_t* __restrict__ first,
                                                  const int32_t* __restrict__ counts,
                                                  float* __restrict__ k, float* __restrict__ v,
-                                                 int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int d = (int)(i % p.hd);
-  const int64_t g = i / p.hd;
-  const int h = (int)(g % p.kv_heads);
-  const int64_t t = g / p.kv_heads;
-  const int b = (int)(t / count), j = (int)(t % count);
-  const int f = first ? first[b] : 0, c = counts ? counts[b] : count;
-  float kx = 0.0f, vx = 0.0f;
-  if (j < c && f >= 0 && f < p.capacity() - j) {
-    const int64_t row = kv_row(s.table + (size_t)b * p.max_pages, f + j, h, p.num_pages, p.kv_heads,
-                               p.page_tokens);
-    if (row >= 0) {
-      const size_t bytes = (size_t)p.pitch * kv_elem_bytes(p.dtype);
-      kx = load_elem(p.k + (size_t)row * bytes, p.dtype, d);
-      vx = load_elem(p.v + (size_t)row * bytes, p.dtype, d);
-      if (p.dtype == kKvE4M3) kx *= p.ks[row], vx *= p.vs[row];
+                                                 int lanes) {
+  RowPlace at;
+  if (!row_place(p, count, lanes, at)) return;
+  const int f = first ? first[at.b] : 0, c = counts ? counts[at.b] : count;
+  v4f kx = {0.f, 0.f, 0.f, 0.f}, vx = kx;
+  if (at.j < c && f >= 0 && f < p.capacity() - at.j) {
+    const int64_t row = kv_row(s.table + (size_t)at.b * p.max_pages, f + at.j, at.h, p.num_pages,
+                               p.kv_heads, p.page_tokens);
+    if (row >= 0 && at.d < p.pitch) {
+      const size_t o = (size_t)row * p.pitch * kv_elem_bytes(DT);
+      kx = read_row4<DT>(p.k + o, at.d);
+      vx = read_row4<DT>(p.v + o, at.d);
+      if constexpr (DT == kKvE4M3) kx *= p.ks[row], vx *= p.vs[row];
     }
   }
-  k[i] = kx;
-  v[i] = vx;
+  const size_t o = (at.t * p.kv_heads + at.h) * (size_t)p.hd;
+  write_row4<VEC>(k + o, kx, at.d, p.hd);
+  write_row4<VEC>(v + o, vx, at.d, p.hd);
 }
 
 // ---------------------------------------------------------------------------
@@ -166,6 +195,7 @@ typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
 
 constexpr float kSlack = 8.0f;
+constexpr int kKvFinishHeads = 64;  // heads whose sums k_kv_finish holds at once
 
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
@@ -207,6 +237,91 @@ struct KvShape {
   static constexpr int KFULL = (kv_hd_below(DT, HDP) * ELEM + 16) / 64;
 };
 
+// Sequence `b` of a call: entries, the query's position, the tiles to take.
+template <int KT>
+__device__ __forceinline__ void kv_sequence(const KvPool& p, const KvSeqs& s, const KvAttend& a, int b,
+                                            int& n, int& qp, int& first, int& tiles) {
+  n = kv_entries(s.lens[b], a.tail, p.capacity());
+  qp = (s.next_pos ? s.next_pos[b] : n - a.tail) + a.tail - 1;
+  first = kv_first_tile(n, qp, s.pos == nullptr ? a.window : 0, KT);
+  tiles = (n + KT - 1) / KT - first;
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor((long long)x, off, 64);
+  return x;
+}
+
+// Inclusive sums over the lanes.
+__device__ __forceinline__ int wave_scan(int x, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off, 64);
+    if (lane >= off) x += y;
+  }
+  return x;
+}
+
+// The part of workgroup blockIdx.x: its sequence, tiles [t0, t1), and where
+// the sequence has more than one part the slot of its sums.
+struct KvPlace {
+  int b, n, qp, t0, t1, index, parts, slot;
+};
+template <int KT>
+__device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const KvAttend& a,
+                                         const KvPart& part, int lane, KvPlace& w) {
+  int first, tiles, step, index = 0;
+  if (s.nseq == 1 || part.target == 0) {
+    // one sequence, or all in one part each
+    w.b = s.nseq == 1 ? 0 : blockIdx.x;
+    kv_sequence<KT>(p, s, a, w.b, w.n, w.qp, first, tiles);
+    step = part.target == 0 ? tiles : kv_part_tiles(tiles, part.target, KT);
+    w.parts = part.target == 0 ? 1 : kv_parts(tiles, step);
+    index = s.nseq == 1 ? blockIdx.x : 0;
+    w.slot = index;
+    if (index >= w.parts) return false;
+  } else {
+    int n = 0, qp = 0, f = 0, t = 0;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < s.nseq; b0 += 64) {
+      t = 0;
+      if (b0 + lane < s.nseq) kv_sequence<KT>(p, s, a, b0 + lane, n, qp, f, t);
+      total += wave_sum(t);
+    }
+    step = kv_part_tiles(total, part.target, KT);
+    int parts_before = 0, slots_before = 0;
+    unsigned long long hit = 0;
+    for (int b0 = 0; b0 < s.nseq; b0 += 64) {
+      const bool in = b0 + lane < s.nseq;
+      if (s.nseq > 64 && in) kv_sequence<KT>(p, s, a, b0 + lane, n, qp, f, t);
+      const int parts = in ? kv_parts(t, step) : 0, slots = parts > 1 ? parts : 0;
+      const int up = wave_scan(parts, lane), sup = wave_scan(slots, lane);
+      const int at = (int)blockIdx.x - parts_before;
+      hit = __ballot(in && at >= up - parts && at < up);
+      if (hit) {
+        const int who = __builtin_ctzll(hit);
+        w.b = b0 + who;
+        w.n = __builtin_amdgcn_readlane(n, who);
+        w.qp = __builtin_amdgcn_readlane(qp, who);
+        first = __builtin_amdgcn_readlane(f, who);
+        tiles = __builtin_amdgcn_readlane(t, who);
+        w.parts = __builtin_amdgcn_readlane(parts, who);
+        index = at - __builtin_amdgcn_readlane(up - parts, who);
+        w.slot = slots_before + __builtin_amdgcn_readlane(sup - slots, who) + index;
+        break;
+      }
+      parts_before += __builtin_amdgcn_readlane(up, 63);
+      slots_before += __builtin_amdgcn_readlane(sup, 63);
+    }
+    if (!hit) return false;
+  }
+  w.index = index;
+  w.t0 = first + index * step;
+  w.t1 = w.t0 + step < first + tiles ? w.t0 + step : first + tiles;
+  return true;
+}
+
 template <int DT, int HDP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ? 1 : 2, 8)))
 void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
@@ -216,18 +331,15 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int group = p.heads / p.kv_heads, chunks = (group + 15) / 16;
-  const int h = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
+  const int h = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
   const int cols = group - 16 * chunk < 16 ? group - 16 * chunk : 16;
   const int head0 = h * group + 16 * chunk;
   const int cap = p.capacity();
-  const int n = kv_entries(s.lens[b], a.tail, cap);
-  const int qp = (s.next_pos ? s.next_pos[b] : n - a.tail) + a.tail - 1;
+  KvPlace place;
+  if (!kv_place<KT>(p, s, a, part, lane, place)) return;
+  const int b = place.b, n = place.n, qp = place.qp, t0 = place.t0, t1 = place.t1;
   const int32_t* table = s.table + (size_t)b * p.max_pages;
   const int32_t* pos = s.pos ? s.pos + ((size_t)b * p.kv_heads + h) * cap : nullptr;
-  const KvRange range = kv_range(n, qp, pos == nullptr ? a.window : 0, KT, part.splits);
-  const int t0 = range.first + (int)blockIdx.x * range.step;
-  const int t1 = t0 + range.step < range.end ? t0 + range.step : range.end;
-  if (blockIdx.x != 0 && t0 >= range.end) return;
 
   // queries: head c's values for this lane's part of the contraction
   const bool col_ok = c < cols;
@@ -510,214 +622,518 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
     }
     __syncthreads();
   }
-  if (wave != 0 || !col_ok) return;
-  const size_t hi = (size_t)b * p.heads + head0 + c;
-  float* to;
-  float f = 1.0f;
-  if (range.parts <= 1) {
-    to = a.out + (int64_t)b * a.out_stride + (int64_t)(head0 + c) * p.hd;
-    f = L == 0.0f ? 0.0f : 1.0f / L;
+  if (part.info && place.index == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    part.info[2 * b] = place.slot, part.info[2 * b + 1] = place.parts;
+  if (place.parts == 1) {
+    if (wave != 0 || !col_ok) return;
+    const size_t head = (size_t)b * p.heads + head0 + c;
     if (g == 0) {
       const float lse2 = L == 0.0f ? -INFINITY : M + __builtin_amdgcn_logf(L);
-      if (a.lse) a.lse[hi] = lse2 * kLn2;
-      if (part.lse2) part.lse2[hi] = lse2;
+      if (a.lse) a.lse[head] = lse2 * kLn2;
+      if (part.lse2) part.lse2[head] = lse2;
     }
-  } else {
-    const size_t at = hi * part.splits + blockIdx.x;
-    to = part.out + at * p.hd;
-    if (g == 0) part.ml[2 * at] = M, part.ml[2 * at + 1] = L;
+    float* out = a.out + (int64_t)b * a.out_stride + (int64_t)(head0 + c) * p.hd;
+    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < T::D; ++d) {
+        const int dim = (4 * g + i) * T::D + d;
+        if (dim < p.hd) out[dim] = acc[d][i] * f;
+      }
+    return;
   }
+
+  // more than one part: this one's sums, for k_kv_finish
+  const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3;
+  const size_t me = ((size_t)place.slot * gridDim.y + blockIdx.y) * most;
+  if (wave != 0 || !col_ok) return;
+  if (g == 0) part.ml[2 * (me + c)] = M, part.ml[2 * (me + c) + 1] = L;
+  float* to = part.out + (me + c) * pitch;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int d = 0; d < T::D; ++d) {
       const int dim = (4 * g + i) * T::D + d;
-      if (dim < p.hd) to[dim] = acc[d][i] * f;
+      if (dim < p.hd) to[dim] = acc[d][i];
     }
 }
 
-// Joins the parts of one (sequence, head).
-__global__ __launch_bounds__(256) void k_kv_join(KvPool p, KvSeqs s, KvAttend a, KvPart part, int kt) {
-  const int j = blockIdx.x, b = blockIdx.y, h = j / (p.heads / p.kv_heads);
-  const int n = kv_entries(s.lens[b], a.tail, p.capacity());
-  const int qp = (s.next_pos ? s.next_pos[b] : n - a.tail) + a.tail - 1;
-  const KvRange range = kv_range(n, qp, s.pos == nullptr ? a.window : 0, kt, part.splits);
-  if (range.parts <= 1) return;
-  (void)h;
-  const size_t hi = (size_t)b * p.heads + j, at = hi * part.splits;
-  float M = -INFINITY, L = 0.0f;
-  for (int i = 0; i < range.parts; ++i) M = fmaxf(M, part.ml[2 * (at + i)]);
-  for (int i = 0; i < range.parts; ++i) {
-    const float mi = part.ml[2 * (at + i)];
-    L += part.ml[2 * (at + i) + 1] * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - M));
+// Reference and sum of a head's weights over its parts, in every lane of the
+// wave. ml: the first part's, `stride` floats from one to the next.
+__device__ __forceinline__ void join_sums(const float* ml, size_t stride, int parts, int lane,
+                                          float& top, float& sum) {
+  top = -INFINITY;
+  for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[i * stride]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  sum = 0.0f;
+  for (int i = lane; i < parts; i += 64) {
+    const float mi = ml[i * stride];
+    sum += ml[i * stride + 1] * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
   }
-  for (int d = threadIdx.x; d < p.hd; d += 256) {
-    float o = 0.0f;
-    for (int i = 0; i < range.parts; ++i) {
-      const float mi = part.ml[2 * (at + i)];
-      o += part.out[(at + i) * p.hd + d] * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - M));
-    }
-    a.out[(int64_t)b * a.out_stride + (int64_t)j * p.hd + d] = L == 0.0f ? 0.0f : o / L;
-  }
-  if (threadIdx.x == 0) {
-    const float lse2 = L == 0.0f ? -INFINITY : M + __builtin_amdgcn_logf(L);
-    if (a.lse) a.lse[hi] = lse2 * kLn2;
-    if (part.lse2) part.lse2[hi] = lse2;
-  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
 }
 
-// Running sums: weight[e] += the weights of the K/V head's query heads, from
-// the scores and the sums of e^score.
-__global__ __launch_bounds__(256) void k_kv_track(KvPool p, KvSeqs s, KvAttend a, KvPart part, int kt) {
-  const int h = blockIdx.y, b = blockIdx.z, cap = p.capacity(), group = p.heads / p.kv_heads;
-  const int n = kv_entries(s.lens[b], a.tail, cap);
-  const int qp = (s.next_pos ? s.next_pos[b] : n - a.tail) + a.tail - 1;
-  const KvRange range = kv_range(n, qp, s.pos == nullptr ? a.window : 0, kt, part.splits);
-  const float* lse2 = part.lse2 + (size_t)b * p.heads + (size_t)h * group;
-  const float* sc = part.scores + ((size_t)b * p.heads + (size_t)h * group) * cap;
-  for (int e = range.first * kt + blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
-    float w = 0.0f;
-    for (int j = 0; j < group; ++j) {
-      const float x = sc[(size_t)j * cap + e];
-      w += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - lse2[j]);
+// What follows the parts, for sequence blockIdx.z and K/V head blockIdx.y:
+// workgroups x < group join the parts of query head x; the others add the
+// heads' weights to the running sums, 1024 entries at a time (the scores are
+// there; a head's sum is formed again from its parts).
+__global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
+  const int group = p.heads / p.kv_heads, chunks = kv_chunks(group);
+  const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3;
+  const size_t rows = (size_t)p.kv_heads * chunks;
+  const int slot = part.info[2 * b], parts = part.info[2 * b + 1];
+  // a head's first part, counted in heads, and the next part's
+  auto first_of = [&](int j) {
+    return ((size_t)slot * rows + (size_t)h * chunks + j / 16) * most + j % 16;
+  };
+  const size_t next = rows * most;
+  if ((int)blockIdx.x < group) {
+    if (parts == 1) return;  // written by the attention itself
+    const int j = blockIdx.x;
+    const size_t base = first_of(j), head = (size_t)b * p.heads + (size_t)h * group + j;
+    // four dims per thread, several teams of threads over the parts
+    const int quads = pitch / 4, teams = 256 / quads;
+    const int team = threadIdx.x / quads, quad = threadIdx.x - team * quads;
+    float top, sum;
+    join_sums(part.ml + 2 * base, 2 * next, parts, lane, top, sum);
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    if (team < teams) {
+#pragma unroll 8
+      for (int i = team; i < parts; i += teams) {
+        const size_t at = base + i * next;
+        const float mi = part.ml[2 * at];
+        const v4f x = *reinterpret_cast<const v4f*>(part.out + at * pitch + 4 * quad);
+        o += x * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
+      }
     }
-    s.weight[((size_t)b * p.kv_heads + h) * cap + e] += w;
+    __shared__ v4f meet[256];
+    meet[threadIdx.x] = o;
+    __syncthreads();
+    if (team != 0) return;
+    for (int k = 1; k < teams; ++k) o += meet[k * quads + quad];
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float* out = a.out + (int64_t)b * a.out_stride + ((int64_t)h * group + j) * p.hd + 4 * quad;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (4 * quad + k < p.hd) out[k] = o[k] * f;
+    if (a.lse && quad == 0)
+      a.lse[head] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    return;
+  }
+  int n, qp, first, tiles;
+  kv_sequence<16>(p, s, a, b, n, qp, first, tiles);
+  const int cap = p.capacity(), e0 = 16 * first + 1024 * ((int)blockIdx.x - group);
+  if (e0 >= n) return;
+  const size_t head = (size_t)b * p.heads + (size_t)h * group;
+  __shared__ float lse2[kKvFinishHeads];
+  const float* sc = part.scores + head * cap;
+  float* weight = s.weight + ((size_t)b * p.kv_heads + h) * cap;
+  const int step = 1024 * ((int)gridDim.x - group);
+  for (int j0 = 0; j0 < group; j0 += kKvFinishHeads) {
+    const int heads = group - j0 < kKvFinishHeads ? group - j0 : kKvFinishHeads;
+    __syncthreads();
+    for (int j = wave; j < heads; j += 4) {
+      float x;
+      if (parts == 1) {
+        x = part.lse2[head + j0 + j];
+      } else {
+        float top, sum;
+        join_sums(part.ml + 2 * first_of(j0 + j), 2 * next, parts, lane, top, sum);
+        x = sum == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+      }
+      if (lane == 0) lse2[j] = x;
+    }
+    __syncthreads();
+    for (int e = e0 + 4 * (int)threadIdx.x; e < n; e += step) {
+      v4f w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int j = 0; j < heads; ++j) {
+        const v4f x = *reinterpret_cast<const v4f*>(sc + (size_t)(j0 + j) * cap + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] += x[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k] - lse2[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + k < n) weight[e + k] += w[k];
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Choice of the entries to keep: the key of the `budget`-th entry bit by bit,
-// then the kept entries from behind the budget into the holes below it, both
-// in index order. One workgroup per (sequence, K/V head).
-constexpr int kChooseThreads = 1024;
+// Choice of the entries to keep, for one K/V head of one sequence: the key
+// (kv_weight_key; sinks and recent entries on top) of the `budget`-th entry by
+// counting the digits of the keys from the top (11, 11 and 10 bits), then the
+// kept entries from behind the budget into the holes below it, both in index
+// order. Counts are whole numbers, so the order in which lanes add them does
+// not matter. Capacities of up to 32768 entries take one workgroup and one
+// launch, the keys held in registers; longer ones segments of 16384 entries
+// with a workgroup each and a launch per step (kLong, below).
+constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
+constexpr int kChooseOne = 32 * kChooseThreads;  // most entries of one workgroup
+constexpr int kDigits = 2048;
+constexpr int kShift[3] = {21, 10, 0};
 
-__device__ __forceinline__ int block_count(bool x, int* red) {
-  const unsigned long long bits = __ballot(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = __popcll(bits);
-  __syncthreads();
-  int n = 0;
-  for (int w = 0; w < kChooseThreads / 64; ++w) n += red[w];
-  return n;
+// What is kept: keys above `least`, and the first `ties` entries at it.
+struct KvCut {
+  uint32_t least;
+  int ties;
+};
+
+// The entries of a workgroup, whole runs of 64 per wave in index order.
+template <int KPT>
+struct KvKeys {
+  uint32_t key[KPT];
+  int first, end, runs;  // entry of run 0, lane 0 of this wave; the end of all; runs per wave
+
+  __device__ __forceinline__ int entry(int i, int lane) const { return first + 64 * i + lane; }
+  __device__ __forceinline__ void load(const KvPool& p, const KvSeqs& s, int b, int h, int sinks,
+                                       int recent, int n, int from, int to, int wave, int lane) {
+    const size_t base = ((size_t)b * p.kv_heads + h) * p.capacity();
+    const float* weight = s.weight + base;
+    const int32_t* pos = s.pos ? s.pos + base : nullptr;
+    const int64_t late = (int64_t)(s.next_pos ? s.next_pos[b] : n) - recent;
+    end = to;
+    runs = (to - from + kChooseThreads - 1) / kChooseThreads;
+    first = from + wave * runs * 64;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const int e = entry(i, lane);
+      key[i] = 0;
+      if (i < runs && e < end) {
+        const int q = pos ? pos[e] : e;
+        key[i] = q < sinks || q >= late ? kKvKeyFirst : kv_weight_key(weight[e]);
+      }
+    }
+  }
+  // f(i, e, in): for every run, with all lanes
+  template <class F>
+  __device__ __forceinline__ void each(int lane, F&& f) const {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i)
+      if (i < runs) f(i, entry(i, lane), entry(i, lane) < end);
+  }
+};
+
+// Counts digit `step` of the keys that agree with `least` above it.
+template <int KPT>
+__device__ __forceinline__ void count_digits(const KvKeys<KPT>& keys, int step, uint32_t least,
+                                             uint32_t* hist, int lane) {
+  keys.each(lane, [&](int i, int, bool in) {
+    const uint32_t k = keys.key[i];
+    const bool on = in && (step == 0 || (k >> kShift[step - 1]) == (least >> kShift[step - 1]));
+    const uint32_t digit = (k >> kShift[step]) & (step == 2 ? 1023u : 2047u);
+    // the lanes that share the first one's digit add once (running sums of 0,
+    // and entries that stay in any case, come in long runs)
+    const unsigned long long act = __ballot(on);
+    if (!act) return;
+    const int lead = __builtin_ctzll(act);
+    const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)digit, lead);
+    const unsigned long long same = __ballot(on && digit == d0);
+    if (lane == lead) atomicAdd(&hist[d0], (uint32_t)__popcll(same));
+    if (on && digit != d0) atomicAdd(&hist[digit], 1u);
+  });
 }
 
-// Flags before this thread's in the workgroup; total: all of them.
-__device__ __forceinline__ int block_rank(bool x, int* red, int& total) {
-  const unsigned long long bits = __ballot(x);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The digit of the need-th key from the top of hist (every thread calls);
+// need becomes its rank among the keys of that digit.
+__device__ __forceinline__ uint32_t find_digit(const uint32_t* hist, int& need, int* red, int tid) {
+  const int lane = tid & 63, wave = tid >> 6;
+  const int c0 = (int)hist[kDigits - 1 - 2 * tid], c1 = (int)hist[kDigits - 2 - 2 * tid];
+  const int up = wave_scan(c0 + c1, lane);
+  if (lane == 63) red[wave] = up;
   __syncthreads();
-  if (lane == 0) red[wave] = __popcll(bits);
+  int before = up - c0 - c1;
+  for (int w = 0; w < kChooseWaves; ++w) before += w < wave ? red[w] : 0;
+  if (before < need && need <= before + c0 + c1) {
+    const bool second = need > before + c0;
+    red[kChooseWaves] = kDigits - 1 - 2 * tid - (second ? 1 : 0);
+    red[kChooseWaves + 1] = need - before - (second ? c0 : 0);
+  }
+  __syncthreads();
+  const uint32_t digit = (uint32_t)red[kChooseWaves];
+  need = red[kChooseWaves + 1];
+  __syncthreads();
+  return digit;
+}
+
+// Sums over the earlier waves of one value per wave; total: of all.
+__device__ __forceinline__ int waves_before(int x, int* red, int wave, int lane, int& total) {
+  __syncthreads();
+  if (lane == 0) red[wave] = x;
   __syncthreads();
   int before = 0;
   total = 0;
-  for (int w = 0; w < kChooseThreads / 64; ++w) {
-    if (w == wave) before = total;
+  for (int w = 0; w < kChooseWaves; ++w) {
+    before += w < wave ? red[w] : 0;
     total += red[w];
   }
-  return before + __popcll(bits & ((1ull << lane) - 1));
+  return before;
 }
 
+// Entries at the cut, and above it, of a wave: below the budget and behind it.
+struct KvCounts {
+  int eq_low = 0, eq_high = 0, up_low = 0, up_high = 0;
+};
+template <int KPT>
+__device__ __forceinline__ KvCounts count_cut(const KvKeys<KPT>& keys, uint32_t least, int budget,
+                                              int lane) {
+  KvCounts c;
+  keys.each(lane, [&](int i, int e, bool in) {
+    const bool eq = in && keys.key[i] == least, up = in && keys.key[i] > least;
+    c.eq_low += __popcll(__ballot(eq && e < budget));
+    c.eq_high += __popcll(__ballot(eq && e >= budget));
+    c.up_low += __popcll(__ballot(up && e < budget));
+    c.up_high += __popcll(__ballot(up && e >= budget));
+  });
+  return c;
+}
+
+// Ranks the holes (hole; -1 elsewhere); WRITE: the kept entries below the
+// budget to src and those behind it to list. eq, holes, tails: how many come
+// before this wave.
+template <int KPT, bool WRITE>
+__device__ __forceinline__ void place_kept(const KvKeys<KPT>& keys, const KvCut& cut, int budget,
+                                           int eq, int holes, int tails, int32_t* src, int32_t* list,
+                                           int (&hole)[KPT], int lane) {
+  const unsigned long long before = (1ull << lane) - 1;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) hole[i] = -1;
+  keys.each(lane, [&](int i, int e, bool in) {
+    const bool at = in && keys.key[i] == cut.least;
+    const unsigned long long ats = __ballot(at);
+    const bool kept = in && (keys.key[i] > cut.least || (at && eq + __popcll(ats & before) < cut.ties));
+    eq += __popcll(ats);
+    const bool low = in && e < budget;
+    const unsigned long long hs = __ballot(low && !kept), ts = __ballot(in && !low && kept);
+    if (low && !kept) hole[i] = holes + __popcll(hs & before);
+    if constexpr (WRITE) {
+      if (low && kept) src[e] = e;
+      if (in && !low && kept) list[tails + __popcll(ts & before)] = e;
+    }
+    holes += __popcll(hs);
+    tails += __popcll(ts);
+  });
+}
+
+// Kept entries at the cut among `eq` with `before` of them in front.
+__device__ __forceinline__ int kept_at_cut(int ties, int before, int eq) {
+  const int left = ties - before;
+  return left < 0 ? 0 : left < eq ? left : eq;
+}
+
+template <int KPT>
 __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvPool p, KvSeqs s, int budget,
                                                               int sinks, int recent,
                                                               int32_t* __restrict__ out) {
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, cap = p.capacity();
-  __shared__ int red[kChooseThreads / 64];
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ uint32_t hist[kDigits];
+  __shared__ int red[kChooseWaves + 2];
+  __shared__ int32_t list[KPT * kChooseThreads / 2];  // of n > budget entries, at most half move
   const int n = kv_entries(s.lens[b], 0, cap);
-  const int end = s.next_pos ? s.next_pos[b] : n;
-  const size_t base = ((size_t)b * p.kv_heads + h) * cap;
-  const float* weight = s.weight + base;
-  const int32_t* pos = s.pos ? s.pos + base : nullptr;
   int32_t* src = out + ((size_t)b * p.kv_heads + h) * budget;
   if (n <= budget) {
     for (int j = tid; j < budget; j += kChooseThreads) src[j] = j < n ? j : -1;
     return;
   }
-  auto key = [&](int e) {
-    const int q = pos ? pos[e] : e;
-    if (q < sinks || (int64_t)q >= (int64_t)end - recent) return kKvKeyFirst;
-    return kv_weight_key(weight[e]);
-  };
-  uint32_t least = 0;  // the largest key that `budget` entries reach
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = least | (1u << bit);
-    int c = 0;
-    for (int e0 = 0; e0 < n; e0 += kChooseThreads)
-      c += block_count(e0 + tid < n && key(e0 + tid) >= t, red);
-    if (c >= budget) least = t;
-  }
-  int above = 0;
-  for (int e0 = 0; e0 < n; e0 += kChooseThreads)
-    above += block_count(e0 + tid < n && key(e0 + tid) > least, red);
-  const int ties = budget - above;  // of the entries at `least`, the first ones
-  int equal = 0;  // entries at `least` below the budget
-  for (int e0 = 0; e0 < budget; e0 += kChooseThreads)
-    equal += block_count(e0 + tid < budget && key(e0 + tid) == least, red);
-  // the kept entries from behind the budget, in order, listed in src from its
-  // start (there are as many holes below the budget: the list fits)
-  int holes = 0, seen = equal;
-  for (int e0 = budget; e0 < n; e0 += kChooseThreads) {
-    const int e = e0 + tid;
-    const uint32_t k = e < n ? key(e) : 0;
-    int total;
-    const int r = block_rank(e < n && k == least, red, total);
-    const bool kept = e < n && (k > least || (k == least && seen + r < ties));
-    seen += total;
-    const int at = block_rank(kept, red, total);
-    if (kept) src[holes + at] = e;
-    holes += total;
-  }
-  // The slots from the last to the first: the hole of rank i takes src[i],
-  // and i is at most its own index, so what a run of slots overwrites is
-  // listed for its own holes (read before) or for those already done.
-  seen = equal;
-  int left = holes;
-  for (int e0 = (budget - 1) / kChooseThreads * kChooseThreads; e0 >= 0; e0 -= kChooseThreads) {
-    const int e = e0 + tid;
-    const bool in = e < budget;
-    const uint32_t k = in ? key(e) : 0;
-    int total;
-    const int r = block_rank(in && k == least, red, total);
-    seen -= total;
-    const bool hole = in && !(k > least || (k == least && seen + r < ties));
-    const int at = block_rank(hole, red, total);
-    left -= total;
-    const int from = hole ? src[left + at] : e;
+  KvKeys<KPT> keys;
+  keys.load(p, s, b, h, sinks, recent, n, 0, n, wave, lane);
+  KvCut cut = {0u, budget};
+#pragma unroll
+  for (int step = 0; step < 3; ++step) {
+    hist[tid] = 0, hist[tid + kChooseThreads] = 0;
     __syncthreads();
-    if (in) src[e] = from;
+    count_digits(keys, step, cut.least, hist, lane);
+    __syncthreads();
+    cut.least |= find_digit(hist, cut.ties, red, tid) << kShift[step];
+  }
+  const KvCounts c = count_cut(keys, cut.least, budget, lane);
+  int total;
+  const int eq = waves_before(c.eq_low + c.eq_high, red, wave, lane, total);
+  const int kept_low = c.up_low + kept_at_cut(cut.ties, eq, c.eq_low);
+  const int kept_high = c.up_high + kept_at_cut(cut.ties, eq + c.eq_low, c.eq_high);
+  int low = budget - keys.first;  // this wave's entries below the budget
+  const int mine = keys.end - keys.first < 64 * keys.runs ? keys.end - keys.first : 64 * keys.runs;
+  low = low < 0 ? 0 : low < mine ? low : mine < 0 ? 0 : mine;
+  const int holes = waves_before(low - kept_low, red, wave, lane, total);
+  const int tails = waves_before(kept_high, red, wave, lane, total);
+  int hole[KPT];
+  place_kept<KPT, true>(keys, cut, budget, eq, holes, tails, src, list, hole, lane);
+  __syncthreads();
+  keys.each(lane, [&](int i, int e, bool) {
+    if (hole[i] >= 0) src[e] = list[hole[i]];
+  });
+}
+
+// Long sequences: every step of the above a launch, a workgroup per segment of
+// kSegment entries. The digits are counted in memory (zero between calls: the
+// last step clears them), the rest follows from the segments' counts.
+constexpr int kSegKeys = 16, kSegment = kSegKeys * kChooseThreads;
+
+struct KvChooseLong {
+  uint32_t* hist;    // [rows][3][kDigits]
+  KvCut* cut;        // [rows]
+  KvCounts* counts;  // [rows][segments]
+  int32_t* list;     // [rows][capacity / 2]
+  int segments, budget, sinks, recent;
+};
+
+// STEP 0-2: count a digit; 3: count what is at and above the cut; 4: write
+// the kept entries and list those behind the budget; 5: fill the holes.
+template <int STEP>
+__global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvSeqs s, KvChooseLong c,
+                                                                   int32_t* __restrict__ out) {
+  const int h = blockIdx.y, b = blockIdx.z, seg = blockIdx.x, tid = threadIdx.x, cap = p.capacity();
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = b * p.kv_heads + h, budget = c.budget;
+  __shared__ uint32_t hist[kDigits];
+  __shared__ int red[kChooseWaves + 2];
+  const int n = kv_entries(s.lens[b], 0, cap);
+  int32_t* src = out + (size_t)row * budget;
+  const int from = seg * kSegment, to = n - from < kSegment ? n : from + kSegment;
+  if (n <= budget) {
+    if (STEP == 4)
+      for (int j = from + tid; j < budget && j < from + kSegment; j += kChooseThreads)
+        src[j] = j < n ? j : -1;
+    return;
+  }
+  if (from >= n) return;
+  KvKeys<kSegKeys> keys;
+  keys.load(p, s, b, h, c.sinks, c.recent, n, from, to, wave, lane);
+  KvCut cut = {0u, budget};
+  uint32_t* rows = c.hist + (size_t)row * 3 * kDigits;
+  if constexpr (STEP <= 3) {
+#pragma unroll
+    for (int step = 0; step < STEP; ++step)
+      cut.least |= find_digit(rows + step * kDigits, cut.ties, red, tid) << kShift[step];
+  }
+  if constexpr (STEP < 3) {
+    hist[tid] = 0, hist[tid + kChooseThreads] = 0;
+    __syncthreads();
+    count_digits(keys, STEP, cut.least, hist, lane);
+    __syncthreads();
+    for (int i = tid; i < kDigits; i += kChooseThreads)
+      if (hist[i]) atomicAdd(rows + STEP * kDigits + i, hist[i]);
+    return;
+  }
+  if constexpr (STEP >= 4) cut = c.cut[row];
+  KvCounts* counts = c.counts + (size_t)row * c.segments;
+  const KvCounts w = count_cut(keys, cut.least, budget, lane);
+  if constexpr (STEP == 3) {
+    KvCounts all;
+    waves_before(w.eq_low, red, wave, lane, all.eq_low);
+    waves_before(w.eq_high, red, wave, lane, all.eq_high);
+    waves_before(w.up_low, red, wave, lane, all.up_low);
+    waves_before(w.up_high, red, wave, lane, all.up_high);
+    if (tid == 0) {
+      counts[seg] = all;
+      if (seg == 0) c.cut[row] = cut;
+    }
+    return;
+  }
+  if constexpr (STEP >= 4) {
+    if (STEP == 4)  // (the digits' counts are read no more)
+      for (int i = seg * kChooseThreads + tid; i < 3 * kDigits;
+           i += (n + kSegment - 1) / kSegment * kChooseThreads)
+        rows[i] = 0;
+    // what lies in the segments before this one
+    int eq0 = 0, holes0 = 0, tails0 = 0;
+    for (int q0 = 0; q0 < seg; q0 += kChooseThreads) {
+      const int q = q0 + tid;
+      KvCounts x;
+      if (q < seg) x = counts[q];
+      const int eqs = x.eq_low + x.eq_high, up = wave_scan(eqs, lane);
+      int total, all;
+      const int before = eq0 + waves_before(__builtin_amdgcn_readlane(up, 63), red, wave, lane, total) +
+                         up - eqs;
+      int low = budget - q * kSegment;
+      low = q >= seg || low < 0 ? 0 : low < kSegment ? low : kSegment;
+      const int hole = low - x.up_low - kept_at_cut(cut.ties, before, x.eq_low);
+      const int tail = x.up_high + kept_at_cut(cut.ties, before + x.eq_low, x.eq_high);
+      waves_before((int)wave_sum(q < seg ? hole : 0), red, wave, lane, all);
+      holes0 += all;
+      waves_before((int)wave_sum(q < seg ? tail : 0), red, wave, lane, all);
+      tails0 += all;
+      eq0 += total;
+    }
+    int total;
+    const int eq = eq0 + waves_before(w.eq_low + w.eq_high, red, wave, lane, total);
+    const int kept_low = w.up_low + kept_at_cut(cut.ties, eq, w.eq_low);
+    const int kept_high = w.up_high + kept_at_cut(cut.ties, eq + w.eq_low, w.eq_high);
+    int low = budget - keys.first;
+    const int mine = keys.end - keys.first < 64 * keys.runs ? keys.end - keys.first : 64 * keys.runs;
+    low = low < 0 ? 0 : low < mine ? low : mine < 0 ? 0 : mine;
+    const int holes = holes0 + waves_before(low - kept_low, red, wave, lane, total);
+    const int tails = tails0 + waves_before(kept_high, red, wave, lane, total);
+    int32_t* list = c.list + (size_t)row * (cap / 2);
+    int hole[kSegKeys];
+    place_kept<kSegKeys, STEP == 4>(keys, cut, budget, eq, holes, tails, src, list, hole, lane);
+    if constexpr (STEP == 5) {
+      keys.each(lane, [&](int i, int e, bool) {
+        if (hole[i] >= 0) src[e] = list[hole[i]];
+      });
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Compaction: one wave per (sequence, K/V head, slot).
+// Compaction: a wave looks at 64 slots and moves the rows of those that get
+// another entry, as many rows at a time as 64 lanes of 16 bytes hold. Sources
+// lie behind the budget and targets below it, so the order is free.
+template <int LANES>  // per row
 __global__ __launch_bounds__(256) void k_kv_compact(KvPool p, KvSeqs s, int budget,
-                                                    const int32_t* __restrict__ src, int64_t n) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
-  const int lane = threadIdx.x & 63;
-  if (i >= n) return;
-  const int j = (int)(i % budget);
-  const int64_t bh = i / budget;
-  const int h = (int)(bh % p.kv_heads), b = (int)(bh / p.kv_heads);
-  const int e = src[i], cap = p.capacity();
-  if (e < budget || e >= cap || j >= cap) return;  // its own, none, or outside
-  const int32_t* table = s.table + (size_t)b * p.max_pages;
-  const int64_t from = kv_row(table, e, h, p.num_pages, p.kv_heads, p.page_tokens);
-  const int64_t to = kv_row(table, j, h, p.num_pages, p.kv_heads, p.page_tokens);
-  if (lane == 0) {
-    const size_t base = (size_t)bh * cap;
-    if (s.weight) s.weight[base + j] = s.weight[base + e];
-    if (s.pos) s.pos[base + j] = s.pos[base + e];
+                                                    const int32_t* __restrict__ src) {
+  const int lane = threadIdx.x & 63, h = blockIdx.y, b = blockIdx.z, cap = p.capacity();
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  const size_t row = (size_t)b * p.kv_heads + h;
+  const int e = j < budget ? src[row * budget + j] : -1;
+  const bool move = e >= budget && e < cap;  // (otherwise its own, none, or outside)
+  int64_t from = -1, to = -1;
+  if (move) {
+    const int32_t* table = s.table + (size_t)b * p.max_pages;
+    from = kv_row(table, e, h, p.num_pages, p.kv_heads, p.page_tokens);
+    to = kv_row(table, j, h, p.num_pages, p.kv_heads, p.page_tokens);
+    if (s.weight) s.weight[row * cap + j] = s.weight[row * cap + e];
+    if (s.pos) s.pos[row * cap + j] = s.pos[row * cap + e];
   }
-  if (from < 0 || to < 0) return;
+  const bool on = from >= 0 && to >= 0;
+  const unsigned long long mask = __ballot(on);
+  const int count = __popcll(mask);
+  if (count == 0) return;
+  if (on && p.dtype == kKvE4M3) p.ks[to] = p.ks[from], p.vs[to] = p.vs[from];
+  // the k-th move's rows to lane k: a permutation of the lanes
+  const int below = __popcll(mask & ((1ull << lane) - 1));
+  const int at = 4 * (on ? below : count + lane - below);
+  const int from_lo = __builtin_amdgcn_ds_permute(at, (int)from), from_hi = __builtin_amdgcn_ds_permute(at, (int)(from >> 32));
+  const int to_lo = __builtin_amdgcn_ds_permute(at, (int)to), to_hi = __builtin_amdgcn_ds_permute(at, (int)(to >> 32));
   const int bytes = p.pitch * kv_elem_bytes(p.dtype);
-  for (int o = 16 * lane; o < bytes; o += 16 * 64) {
-    *reinterpret_cast<v4f*>(p.k + (size_t)to * bytes + o) =
-        *reinterpret_cast<const v4f*>(p.k + (size_t)from * bytes + o);
-    *reinterpret_cast<v4f*>(p.v + (size_t)to * bytes + o) =
-        *reinterpret_cast<const v4f*>(p.v + (size_t)from * bytes + o);
-  }
-  if (p.dtype == kKvE4M3 && lane == 0) {
-    p.ks[to] = p.ks[from];
-    p.vs[to] = p.vs[from];
+  constexpr int TEAMS = 64 / LANES, AHEAD = 4;
+  const int team = lane / LANES, o = 16 * (lane % LANES);
+  for (int k0 = 0; k0 < count; k0 += TEAMS * AHEAD) {
+    v4f kx[AHEAD], vx[AHEAD];
+    int64_t dst[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = k0 + u * TEAMS + team, who = k < 64 ? k : 63;
+      const int64_t f = ((int64_t)__shfl(from_hi, who, 64) << 32) | (uint32_t)__shfl(from_lo, who, 64);
+      const int64_t t = ((int64_t)__shfl(to_hi, who, 64) << 32) | (uint32_t)__shfl(to_lo, who, 64);
+      dst[u] = k < count && o < bytes ? t * bytes + o : -1;
+      if (dst[u] >= 0) {
+        kx[u] = *reinterpret_cast<const v4f*>(p.k + f * bytes + o);
+        vx[u] = *reinterpret_cast<const v4f*>(p.v + f * bytes + o);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (dst[u] >= 0) {
+        *reinterpret_cast<v4f*>(p.k + dst[u]) = kx[u];
+        *reinterpret_cast<v4f*>(p.v + dst[u]) = vx[u];
+      }
   }
 }
 
@@ -757,39 +1173,83 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
     WV_TRY(c->scores.alloc((size_t)max_seqs * heads * p.capacity() * sizeof(float)));
     WV_TRY(c->lse2.alloc((size_t)max_seqs * heads * sizeof(float)));
   }
-  // every call's parts fit: splits * nseq * kv_heads * chunks stays below the
-  // workgroups that the rule aims at wherever there is more than one part
-  const size_t parts = (size_t)kKvWorkgroups * 16;
-  WV_TRY(c->part.alloc(parts * hd * sizeof(float)));
-  WV_TRY(c->part_ml.alloc(parts * 2 * sizeof(float)));
+  const int chunk_rows = kv_heads * kv_chunks(heads / kv_heads);
+  const int most = heads / kv_heads < 16 ? heads / kv_heads : 16;
+  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows)) * chunk_rows * most;
+  WV_TRY(c->part.alloc(slots * ((hd + 3) & ~3) * sizeof(float)));
+  WV_TRY(c->part_ml.alloc(slots * 2 * sizeof(float)));
+  WV_TRY(c->info.alloc((size_t)max_seqs * 2 * sizeof(int32_t)));
+  if (track && p.capacity() > kChooseOne) {
+    const size_t choose_rows = (size_t)max_seqs * kv_heads;
+    WV_TRY(c->choose_hist.alloc(choose_rows * 3 * kDigits * sizeof(uint32_t)));
+    WV_HIP(hipMemsetAsync(c->choose_hist.p, 0, c->choose_hist.bytes, st));
+    WV_TRY(c->choose_cut.alloc(choose_rows * sizeof(KvCut)));
+    const size_t segments = (p.capacity() + kSegment - 1) / kSegment;
+    WV_TRY(c->choose_counts.alloc(choose_rows * segments * sizeof(KvCounts)));
+    WV_TRY(c->choose_list.alloc(choose_rows * (p.capacity() / 2) * sizeof(int32_t)));
+  }
   WV_HIP(hipStreamSynchronize(st));
   p.k = c->k.as<uint8_t>(), p.v = c->v.as<uint8_t>();
   p.ks = c->ks.as<float>(), p.vs = c->vs.as<float>();
   return Status::ok();
 }
 
-Status launch_kv_append(const KvPool& p, const KvSeqs& s, const KvRows& r, hipStream_t st) {
-  if (s.nseq == 0 || r.rows == 0) return Status::ok();
+// Lanes that take a row, four elements each, and the grid over the rows of
+// every sequence.
+int row_lanes(const KvPool& p) {
   int lanes = 1;
   while (4 * lanes < p.pitch) lanes *= 2;
-  const int64_t groups = (int64_t)s.nseq * r.rows * p.kv_heads;
-  const int64_t blocks = blocks_of(groups * lanes);
-  if (blocks > INT32_MAX) return Status::err(kInvalid, "kv append: too many rows in one call");
+  return lanes;
+}
+Status row_grid(const KvPool& p, int nseq, int rows, int lanes, dim3* grid) {
+  const int64_t threads = (int64_t)rows * p.kv_heads * lanes;
+  if (threads > INT32_MAX)
+    return Status::err(kInvalid, "kv: rows * num_kv_heads * head_dim of one sequence too large");
+  *grid = dim3((unsigned)blocks_of(threads), (unsigned)nseq);
+  return Status::ok();
+}
+
+template <int DT>
+void append_of(bool vec, dim3 grid, const KvPool& p, const KvSeqs& s, const KvRows& r, int lanes,
+               hipStream_t st) {
+  if (vec)
+    k_kv_append<DT, true><<<grid, 256, 0, st>>>(p, s, r, lanes);
+  else
+    k_kv_append<DT, false><<<grid, 256, 0, st>>>(p, s, r, lanes);
+}
+
+Status launch_kv_append(const KvPool& p, const KvSeqs& s, const KvRows& r, hipStream_t st) {
+  if (s.nseq == 0 || r.rows == 0) return Status::ok();
+  const int lanes = row_lanes(p);
+  dim3 grid;
+  WV_TRY(row_grid(p, s.nseq, r.rows, lanes, &grid));
   const bool vec = p.hd % 4 == 0 && r.k_stride % 4 == 0 && r.v_stride % 4 == 0 &&
                    ((uintptr_t)r.k | (uintptr_t)r.v) % 16 == 0;
-  if (vec)
-    k_kv_append<true><<<(unsigned)blocks, 256, 0, st>>>(p, s, r, lanes, groups);
-  else
-    k_kv_append<false><<<(unsigned)blocks, 256, 0, st>>>(p, s, r, lanes, groups);
+  if (p.dtype == kKvF32) append_of<kKvF32>(vec, grid, p, s, r, lanes, st);
+  else if (p.dtype == kKvBF16) append_of<kKvBF16>(vec, grid, p, s, r, lanes, st);
+  else append_of<kKvE4M3>(vec, grid, p, s, r, lanes, st);
   return hip_status(hipGetLastError(), "k_kv_append");
+}
+
+template <int DT>
+void read_of(bool vec, dim3 grid, const KvPool& p, const KvSeqs& s, int count, const int32_t* first,
+             const int32_t* counts, float* k, float* v, int lanes, hipStream_t st) {
+  if (vec)
+    k_kv_read<DT, true><<<grid, 256, 0, st>>>(p, s, count, first, counts, k, v, lanes);
+  else
+    k_kv_read<DT, false><<<grid, 256, 0, st>>>(p, s, count, first, counts, k, v, lanes);
 }
 
 Status launch_kv_read(const KvPool& p, const KvSeqs& s, int count, const int32_t* first,
                       const int32_t* counts, float* k, float* v, hipStream_t st) {
-  const int64_t n = (int64_t)s.nseq * count * p.kv_heads * p.hd;
-  if (n == 0) return Status::ok();
-  if (blocks_of(n) > INT32_MAX) return Status::err(kInvalid, "kv read: too many entries in one call");
-  k_kv_read<<<(unsigned)blocks_of(n), 256, 0, st>>>(p, s, count, first, counts, k, v, n);
+  if (s.nseq == 0 || count == 0) return Status::ok();
+  const int lanes = row_lanes(p);
+  dim3 grid;
+  WV_TRY(row_grid(p, s.nseq, count, lanes, &grid));
+  const bool vec = p.hd % 4 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+  if (p.dtype == kKvF32) read_of<kKvF32>(vec, grid, p, s, count, first, counts, k, v, lanes, st);
+  else if (p.dtype == kKvBF16) read_of<kKvBF16>(vec, grid, p, s, count, first, counts, k, v, lanes, st);
+  else read_of<kKvE4M3>(vec, grid, p, s, count, first, counts, k, v, lanes, st);
   return hip_status(hipGetLastError(), "k_kv_read");
 }
 
@@ -817,42 +1277,71 @@ Status launch_attend(int hd, dim3 grid, const KvPool& p, const KvSeqs& s, const 
 Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream_t st) {
   if (s.nseq == 0) return Status::ok();
   const KvPool& p = c.pool;
-  const int kt = p.dtype == kKvF32 ? 16 : 32;
+  const int rows = p.kv_heads * kv_chunks(p.heads / p.kv_heads);
   KvPart part;
-  part.splits = kv_splits(s.nseq, p.kv_heads, p.heads / p.kv_heads, p.capacity());
+  part.target = kv_target(rows);
+  int64_t parts = kv_most_parts(s.nseq, part.target, p.capacity());
+  if (parts <= s.nseq) part.target = 0, parts = s.nseq;
   part.out = c.part.as<float>();
   part.ml = c.part_ml.as<float>();
+  const bool finish = part.target != 0 || s.weight;
+  if (finish) part.info = c.info.as<int32_t>();
   if (s.weight) {
     part.scores = c.scores.as<float>();
     part.lse2 = c.lse2.as<float>();
   }
-  const dim3 grid(part.splits, p.kv_heads * kv_chunks(p.heads / p.kv_heads), s.nseq);
+  const dim3 grid((unsigned)parts, (unsigned)rows);
   WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, grid, p, s, a, part, st)
          : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, grid, p, s, a, part, st)
                               : launch_attend<kKvE4M3>(p.hd, grid, p, s, a, part, st));
-  if (part.splits > 1) {
-    k_kv_join<<<dim3(p.heads, s.nseq), 256, 0, st>>>(p, s, a, part, kt);
-    WV_TRY(hip_status(hipGetLastError(), "k_kv_join"));
-  }
-  if (!s.weight) return Status::ok();
-  const int blocks = (p.capacity() + 255) / 256;
-  k_kv_track<<<dim3(blocks < 64 ? blocks : 64, p.kv_heads, s.nseq), 256, 0, st>>>(p, s, a, part, kt);
-  return hip_status(hipGetLastError(), "k_kv_track");
+  if (!finish) return Status::ok();
+  const int most = (p.capacity() + 1023) / 1024;
+  const int track = !s.weight ? 0 : most < 64 ? most : 64;
+  k_kv_finish<<<dim3(p.heads / p.kv_heads + track, p.kv_heads, s.nseq), 256, 0, st>>>(p, s, a, part);
+  return hip_status(hipGetLastError(), "k_kv_finish");
 }
 
-Status launch_kv_choose(const KvPool& p, const KvSeqs& s, int budget, int sinks, int recent,
-                        int32_t* src, hipStream_t st) {
+Status kv_choose(const KvCache& c, const KvSeqs& s, int budget, int sinks, int recent, int32_t* src,
+                 hipStream_t st) {
   if (s.nseq == 0) return Status::ok();
-  k_kv_choose<<<dim3(p.kv_heads, s.nseq), kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
+  const KvPool& p = c.pool;
+  const dim3 grid(p.kv_heads, s.nseq);
+  const int cap = p.capacity();
+  if (cap <= 4 * kChooseThreads)
+    k_kv_choose<4><<<grid, kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
+  else if (cap <= 16 * kChooseThreads)
+    k_kv_choose<16><<<grid, kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
+  else if (cap <= kChooseOne)
+    k_kv_choose<32><<<grid, kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
+  else {
+    KvChooseLong l;
+    l.segments = (cap + kSegment - 1) / kSegment;
+    l.budget = budget, l.sinks = sinks, l.recent = recent;
+    l.hist = c.choose_hist.as<uint32_t>();
+    l.cut = c.choose_cut.as<KvCut>();
+    l.counts = c.choose_counts.as<KvCounts>();
+    l.list = c.choose_list.as<int32_t>();
+    const dim3 g(l.segments, p.kv_heads, s.nseq);
+    k_kv_choose_long<0><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+    k_kv_choose_long<1><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+    k_kv_choose_long<2><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+    k_kv_choose_long<3><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+    k_kv_choose_long<4><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+    k_kv_choose_long<5><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+  }
   return hip_status(hipGetLastError(), "k_kv_choose");
 }
 
 Status launch_kv_compact(const KvPool& p, const KvSeqs& s, int budget, const int32_t* src,
                          hipStream_t st) {
-  const int64_t n = (int64_t)s.nseq * p.kv_heads * budget;
-  if (n == 0) return Status::ok();
-  if (blocks_of(n * 64) > INT32_MAX) return Status::err(kInvalid, "kv compact: too many slots in one call");
-  k_kv_compact<<<(unsigned)blocks_of(n * 64), 256, 0, st>>>(p, s, budget, src, n);
+  if (s.nseq == 0) return Status::ok();
+  const dim3 grid((unsigned)blocks_of(budget), p.kv_heads, s.nseq);
+  const int pieces = p.pitch * kv_elem_bytes(p.dtype) / 16;  // at most 64
+  if (pieces <= 4) k_kv_compact<4><<<grid, 256, 0, st>>>(p, s, budget, src);
+  else if (pieces <= 8) k_kv_compact<8><<<grid, 256, 0, st>>>(p, s, budget, src);
+  else if (pieces <= 16) k_kv_compact<16><<<grid, 256, 0, st>>>(p, s, budget, src);
+  else if (pieces <= 32) k_kv_compact<32><<<grid, 256, 0, st>>>(p, s, budget, src);
+  else k_kv_compact<64><<<grid, 256, 0, st>>>(p, s, budget, src);
   return hip_status(hipGetLastError(), "k_kv_compact");
 }
 
