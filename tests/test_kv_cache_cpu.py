@@ -25,6 +25,7 @@ def rules():
     L.kv_check_row.restype = ctypes.c_longlong
     for name in ("most_parts", "most_slots"):
         getattr(L, "kv_check_" + name).restype = ctypes.c_longlong
+    L.kv_check_runs.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     L.kv_check_part_tiles.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
     L.kv_check_scale.restype = ctypes.c_float
     L.kv_check_scale.argtypes = [ctypes.c_float]
@@ -148,12 +149,21 @@ def test_parts_fit_the_grid_and_the_scratch(rules):
         if rng.random() < 0.5:  # a few long ones
             lens = np.where(rng.random(nseq) < 0.1, lens, lens // 50)
         tiles = [-(-int(n) // kt) for n in lens]
-        target = rules.kv_check_target(rows)
-        step = rules.kv_check_part_tiles(sum(tiles), target, kt)
-        parts = [rules.kv_check_parts(t, step) for t in tiles]
-        assert all(p >= 1 and (p - 1) * step < max(t, 1) <= p * step for p, t in zip(parts, tiles))
-        assert sum(parts) <= rules.kv_check_most_parts(nseq, target, cap)
-        assert sum(p for p in parts if p > 1) < max(1, rules.kv_check_most_slots(target))
+        units = [max(1, t) for t in tiles]
+        target = rules.kv_check_target(rows, int(rng.integers(1, 257)))
+        step = rules.kv_check_part_tiles(sum(units), target, kt)
+        most, slots = rules.kv_check_most_parts(nseq, target, cap), rules.kv_check_most_slots(target)
+        if rules.kv_check_runs(sum(units), target, kt):
+            groups = -(-sum(units) // step)
+            assert groups <= min(target, most) and 2 * groups <= slots
+        else:
+            parts = [rules.kv_check_parts(t, step) for t in tiles]
+            assert all(p >= 1 and (p - 1) * step < max(t, 1) <= p * step for p, t in zip(parts, tiles))
+            assert sum(parts) <= most
+            assert sum(p for p in parts if p > 1) <= slots
+        # one sequence by itself
+        step = rules.kv_check_part_tiles(tiles[0], target, kt)
+        assert rules.kv_check_parts(tiles[0], step) <= min(target, rules.kv_check_most_parts(1, target, cap))
 
 
 def test_first_tile_of_a_window(rules):

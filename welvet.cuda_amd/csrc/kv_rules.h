@@ -65,34 +65,41 @@ constexpr uint32_t kKvKeyFirst = 0xFFFFFFFFu;  // sinks and recent entries
 // Query heads of one K/V head are taken 16 at a time.
 WV_HD int kv_chunks(int group) { return (group + 15) / 16; }
 
-// The attention's workgroups take parts of the sequences' entries, in tiles of
-// `kt`. The parts of all sequences are alike: about `target` of them would
-// take every tile (kv_part_tiles), so that unequal sequences keep the GPU
-// evenly busy; a sequence has one at least. `target` counts the parts per K/V
-// head and chunk of its query heads.
-constexpr int kKvWorkgroups = 512;  // two per CU: 4 waves of up to 256 registers
-WV_HD int kv_target(int kv_rows) {
-  const int n = kKvWorkgroups / kv_rows;
+// Waves per SIMD that the attention kernels' registers leave room for, by
+// head dims.
+WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 1; }
+
+// Workgroups (4 waves) per row (K/V head and chunk of query heads) that fill
+// 256 CUs once, and the tiles of `kt` entries that each takes of `tiles` (one
+// at least per sequence): two for each wave, so that short sequences run side
+// by side, or an equal share. Shares of eight for each wave and more are runs
+// that go over the sequences' ends.
+WV_HD int kv_target(int kv_rows, int hd) {
+  const int n = 256 * kv_waves(hd) / kv_rows;
   return n > 1 ? n : 1;
 }
-constexpr int kKvLeastEntries = 256;  // two tiles for each of a workgroup's waves
+constexpr int kKvLeastEntries = 256;
 WV_HD int kv_part_tiles(int64_t tiles, int target, int kt) {
   const int64_t n = (tiles + target - 1) / target;
   return n > kKvLeastEntries / kt ? (int)n : kKvLeastEntries / kt;
+}
+WV_HD bool kv_runs(int64_t tiles, int target, int kt) {
+  return kv_part_tiles(tiles, target, kt) > 4 * (kKvLeastEntries / kt);
 }
 WV_HD int kv_parts(int tiles, int part_tiles) {
   const int n = (tiles + part_tiles - 1) / part_tiles;
   return n > 1 ? n : 1;
 }
-// Most parts of all sequences: every tile in part_tiles' share, and one that
-// is not full per sequence.
+// Most workgroups of a row: full parts, and one that is not full per sequence;
+// a sequence's parts hold kKvLeastEntries at least but for its last.
 WV_HD int64_t kv_most_parts(int nseq, int target, int capacity) {
   const int64_t by_target = (int64_t)target + nseq;
   const int64_t by_capacity = (int64_t)nseq * ((capacity + kKvLeastEntries - 1) / kKvLeastEntries);
   return by_target < by_capacity ? by_target : by_capacity;
 }
-// Most parts of the sequences that have more than one: their tiles exceed a
-// part each, so there are fewer than `target` of them.
+// Most slots of a row for the sums of sequences of more than one part: two per
+// run (the end of one sequence and the start of another); without runs, there
+// are at most `target` full parts, and these sequences have one or more each.
 WV_HD int64_t kv_most_slots(int target) { return 2 * (int64_t)target; }
 
 // First tile of `kt` entries that a window over indices leaves (0: no window).

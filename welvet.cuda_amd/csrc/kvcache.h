@@ -68,13 +68,17 @@ struct KvAttend {
 // How an attention call is cut, and its scratch. ml and out: per slot (a part
 // of a sequence of more than one), row of query heads (K/V head and chunk of
 // 16 heads) and head the reference and sum of the weights and the unscaled
-// sums of V; info: a sequence's first slot and number of parts; scores (log2
-// units) and lse2: for the running sums, null without.
+// sums of V; scores (log2 units) and lse2: for the running sums, null without.
+// Part 0 of a sequence has `slot`, part i > 0 slot + 1 + (i - 1) stride.
+struct KvInfo {
+  int slot, parts, stride;
+};
 struct KvPart {
   int target = 0;             // kv_target; 0: every sequence is one part
+  bool vec_q = false, vec_out = false;  // rows of q and out hold whole 16-byte pieces
   float* out = nullptr;       // [slots][rows][heads of a row][hd up to 4]
   float* ml = nullptr;        // [slots][rows][heads of a row][2]
-  int32_t* info = nullptr;    // [nseq][2], null where nothing follows the parts
+  KvInfo* info = nullptr;     // [nseq], null where nothing follows the parts
   float* scores = nullptr;    // [nseq][heads][capacity]
   float* lse2 = nullptr;      // [nseq][heads]
 };

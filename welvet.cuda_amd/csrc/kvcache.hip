@@ -12,6 +12,7 @@
 #include "kvcache.h"
 
 #include "bf16.h"
+#include "wave.h"
 
 namespace wv {
 namespace {
@@ -197,20 +198,24 @@ typedef uint32_t u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
 constexpr float kSlack = 8.0f;
 constexpr int kKvFinishHeads = 64;  // heads whose sums k_kv_finish holds at once
 
+// A piece of a V row. (Non-temporal: V lines are read whole by one instruction,
+// and K lines by two, which keeps the ones of K in the caches between the two:
+// 1 x 131072 entries of 8 heads of 128 in bf16 105.7 us with plain loads of
+// both, 87.9 with these of V, 88.3 of K instead, 95.3 of both.)
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
   int i = 0;
 #pragma unroll
   for (; i + 4 <= N; i += 4) {
-    const u32x4 x = *reinterpret_cast<const u32x4_a4*>(p + 4 * i);
+    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a4*>(p + 4 * i));
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[i + k] = x[k];
   }
   if constexpr (N % 4 >= 2) {
-    const auto x = *reinterpret_cast<const u32x2_a4*>(p + 4 * (N / 4 * 4));
+    const auto x = __builtin_nontemporal_load(reinterpret_cast<const u32x2_a4*>(p + 4 * (N / 4 * 4)));
     w[N / 4 * 4] = x[0], w[N / 4 * 4 + 1] = x[1];
   }
-  if constexpr (N % 2 == 1) w[N - 1] = *reinterpret_cast<const uint32_t*>(p + 4 * (N - 1));
+  if constexpr (N % 2 == 1) w[N - 1] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + 4 * (N - 1)));
 }
 
 // Two E4M3 codes (the low or the high half of w) as two bf16.
@@ -247,37 +252,67 @@ __device__ __forceinline__ void kv_sequence(const KvPool& p, const KvSeqs& s, co
   tiles = (n + KT - 1) / KT - first;
 }
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor((long long)x, off, 64);
-  return x;
+// x of the lane that a DPP control names, 0 where there is none.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int dpp_or_0(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
 }
 
-// Inclusive sums over the lanes.
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
+// Inclusive sums over the lanes, by moves within rows of 16 and from the last
+// lane of a row to the rows behind it (VALU operations, no LDS round trips).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_or_0<0x111>(x);       // row_shr:1
+  x += dpp_or_0<0x112>(x);       // row_shr:2
+  x += dpp_or_0<0x114>(x);       // row_shr:4
+  x += dpp_or_0<0x118>(x);       // row_shr:8
+  x += dpp_or_0<0x142, 0xA>(x);  // row_bcast:15 to rows 1 and 3
+  x += dpp_or_0<0x143, 0xC>(x);  // row_bcast:31 to rows 2 and 3
   return x;
 }
+__device__ __forceinline__ int wave_sum(int x) {
+  return __builtin_amdgcn_readlane(wave_scan(x), 63);
+}
 
-// The part of workgroup blockIdx.x: its sequence, tiles [t0, t1), and where
-// the sequence has more than one part the slot of its sums.
+// The tiles of workgroup blockIdx.x: [t0, t1) of sequence b, which has `parts`
+// of them (index 0: its first), and where these are more than one the slot of
+// its sums (KvInfo). Three ways to cut:
+//   target 0: every sequence is one part;
+//   parts of `step` tiles of one sequence each;
+//   RUNS, many tiles: runs of `step` tiles over all sequences one after the
+//   other, the same for every workgroup however unequal the sequences are (64
+//   sequences of 512 to 4096 E4M3 entries, 32 heads over 8 of 128: parts 81.7
+//   us, runs 77.0). A workgroup then ends one sequence, may take whole ones
+//   (left: its tiles still to come) and starts another: two slots each. Few
+//   tiles are better off with parts, which a workgroup is sooner done with (16
+//   sequences of up to 8191, 12 heads over 4 of 64 with running sums: parts
+//   25.8 us, runs 29.4).
 struct KvPlace {
-  int b, n, qp, t0, t1, index, parts, slot;
+  int b, n, qp, t0, t1, index, parts, slot, stride, left, step;
 };
-template <int KT>
+
+// The tiles of a run that starts at tile `off` of sequence w.b.
+__device__ __forceinline__ void kv_run(int first, int tiles, int off, KvPlace& w) {
+  const int units = tiles > 1 ? tiles : 1;  // (one for a sequence without tiles)
+  w.t0 = first + off;
+  w.t1 = units - off < w.left ? first + tiles : w.t0 + w.left;
+  if (w.t1 > first + tiles) w.t1 = first + tiles;
+  w.index = off > 0 ? 1 : 0;
+  const int behind = units - off - w.left;  // tiles of the sequence for later workgroups
+  w.parts = off > 0 ? 2 : behind > 0 ? 1 + (behind + w.step - 1) / w.step : 1;
+  w.slot = 2 * (int)blockIdx.x + (off > 0 ? 0 : 1);
+  w.left = behind < 0 ? -behind : 0;
+}
+
+template <int KT, bool RUNS>
 __device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const KvAttend& a,
                                          const KvPart& part, int lane, KvPlace& w) {
-  int first, tiles, step, index = 0;
+  int first, tiles, index = 0;
+  w.left = 0, w.stride = 1;
   if (s.nseq == 1 || part.target == 0) {
-    // one sequence, or all in one part each
     w.b = s.nseq == 1 ? 0 : blockIdx.x;
     kv_sequence<KT>(p, s, a, w.b, w.n, w.qp, first, tiles);
-    step = part.target == 0 ? tiles : kv_part_tiles(tiles, part.target, KT);
-    w.parts = part.target == 0 ? 1 : kv_parts(tiles, step);
+    w.step = part.target == 0 ? tiles : kv_part_tiles(tiles, part.target, KT);
+    w.parts = part.target == 0 ? 1 : kv_parts(tiles, w.step);
     index = s.nseq == 1 ? blockIdx.x : 0;
     w.slot = index;
     if (index >= w.parts) return false;
@@ -286,19 +321,48 @@ __device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const
     int64_t total = 0;
     for (int b0 = 0; b0 < s.nseq; b0 += 64) {
       t = 0;
-      if (b0 + lane < s.nseq) kv_sequence<KT>(p, s, a, b0 + lane, n, qp, f, t);
-      total += wave_sum(t);
+      const bool in = b0 + lane < s.nseq;
+      if (in) kv_sequence<KT>(p, s, a, b0 + lane, n, qp, f, t);
+      // (halves, so that a wave's sum of up to 2^26 tiles each fits)
+      const int units = in ? (t > 1 ? t : 1) : 0;
+      total += wave_sum(units & 0xFFFF) + ((int64_t)wave_sum(units >> 16) << 16);
     }
-    step = kv_part_tiles(total, part.target, KT);
+    w.step = kv_part_tiles(total, part.target, KT);
+    const bool runs = RUNS && kv_runs(total, part.target, KT);
+    const int64_t start = (int64_t)blockIdx.x * w.step;
+    if (runs && start >= total) return false;
+    int64_t units_before = 0;
     int parts_before = 0, slots_before = 0;
     unsigned long long hit = 0;
     for (int b0 = 0; b0 < s.nseq; b0 += 64) {
       const bool in = b0 + lane < s.nseq;
       if (s.nseq > 64 && in) kv_sequence<KT>(p, s, a, b0 + lane, n, qp, f, t);
-      const int parts = in ? kv_parts(t, step) : 0, slots = parts > 1 ? parts : 0;
-      const int up = wave_scan(parts, lane), sup = wave_scan(slots, lane);
-      const int at = (int)blockIdx.x - parts_before;
-      hit = __ballot(in && at >= up - parts && at < up);
+      if (runs) {
+        const int units = in ? (t > 1 ? t : 1) : 0;
+        const int64_t up = wave_scan(units & 0xFFFF) + ((int64_t)wave_scan(units >> 16) << 16);
+        const int64_t at = start - units_before;
+        hit = __ballot(in && at >= up - units && at < up);
+        const int who = hit ? __builtin_ctzll(hit) : 63;
+        // (what the lane before has)
+        const int64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)up, who);
+        const int64_t all = lo | ((int64_t)__builtin_amdgcn_readlane((int)(up >> 32), who) << 32);
+        if (hit) index = (int)(at - (all - __builtin_amdgcn_readlane(units, who)));
+        units_before += all;
+      } else {
+        const int parts = in ? kv_parts(t, w.step) : 0;
+        const int up = wave_scan(parts);
+        const unsigned long long ones = __ballot(parts == 1);  // (they take no slots)
+        const int at = (int)blockIdx.x - parts_before;
+        hit = __ballot(in && at >= up - parts && at < up);
+        if (hit) {
+          const int who = __builtin_ctzll(hit);
+          w.parts = __builtin_amdgcn_readlane(parts, who);
+          index = at - __builtin_amdgcn_readlane(up - parts, who);
+          w.slot = slots_before + at - (int)__popcll(ones & ((1ull << who) - 1));
+        }
+        parts_before += __builtin_amdgcn_readlane(up, 63);
+        slots_before += __builtin_amdgcn_readlane(up, 63) - (int)__popcll(ones);
+      }
       if (hit) {
         const int who = __builtin_ctzll(hit);
         w.b = b0 + who;
@@ -306,24 +370,37 @@ __device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const
         w.qp = __builtin_amdgcn_readlane(qp, who);
         first = __builtin_amdgcn_readlane(f, who);
         tiles = __builtin_amdgcn_readlane(t, who);
-        w.parts = __builtin_amdgcn_readlane(parts, who);
-        index = at - __builtin_amdgcn_readlane(up - parts, who);
-        w.slot = slots_before + __builtin_amdgcn_readlane(sup - slots, who) + index;
         break;
       }
-      parts_before += __builtin_amdgcn_readlane(up, 63);
-      slots_before += __builtin_amdgcn_readlane(sup, 63);
     }
     if (!hit) return false;
+    if (runs) {
+      w.left = w.step, w.stride = 2;
+      kv_run(first, tiles, index, w);
+      return true;
+    }
   }
   w.index = index;
-  w.t0 = first + index * step;
-  w.t1 = w.t0 + step < first + tiles ? w.t0 + step : first + tiles;
+  w.t0 = first + index * w.step;
+  w.t1 = w.t0 + w.step < first + tiles ? w.t0 + w.step : first + tiles;
   return true;
 }
 
-template <int DT, int HDP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ? 1 : 2, 8)))
+// The next sequence of a workgroup's run.
+template <int KT>
+__device__ __forceinline__ bool kv_next(const KvPool& p, const KvSeqs& s, const KvAttend& a, KvPlace& w) {
+  if (w.left == 0 || w.b + 1 >= s.nseq) return false;
+  ++w.b;
+  int first, tiles;
+  kv_sequence<KT>(p, s, a, w.b, w.n, w.qp, first, tiles);
+  kv_run(first, tiles, 0, w);
+  return true;
+}
+
+// GEN: ALiBi, windows, or scores for the running sums. RUNS: workgroups may take
+// runs over several sequences.
+template <int DT, int HDP, bool GEN, bool RUNS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kv_waves(HDP), 8)))
 void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   using T = KvShape<DT, HDP>;
   constexpr int NSUB = T::NSUB, KT = 16 * NSUB, W = 4;
@@ -336,57 +413,15 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   const int head0 = h * group + 16 * chunk;
   const int cap = p.capacity();
   KvPlace place;
-  if (!kv_place<KT>(p, s, a, part, lane, place)) return;
+  if (!kv_place<KT, RUNS>(p, s, a, part, lane, place)) return;
+  constexpr int STRIDE = HDP + 4;
+  constexpr int QBYTES = DT == kKvF32 ? 0 : T::KS * 3 * 1024, SBYTES = W * 16 * STRIDE * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[QBYTES > SBYTES ? QBYTES : SBYTES];
+  __shared__ float ml[W][16][2];
+  do {
   const int b = place.b, n = place.n, qp = place.qp, t0 = place.t0, t1 = place.t1;
   const int32_t* table = s.table + (size_t)b * p.max_pages;
   const int32_t* pos = s.pos ? s.pos + ((size_t)b * p.kv_heads + h) * cap : nullptr;
-
-  // queries: head c's values for this lane's part of the contraction
-  const bool col_ok = c < cols;
-  const float* qrow = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + (col_ok ? c : 0)) * p.hd;
-  const float slope =
-      a.alibi ? (float)(exp2(-8.0 * (double)(head0 + c + 1) / (double)p.heads) * kLog2e) : 0.0f;
-  auto q_at = [&](int d) { return col_ok && d < p.hd ? qrow[d] : 0.0f; };
-  float mult = a.scale2;
-  float qf[DT == kKvF32 ? HDP / 4 : 1];
-  bf16x8 qt[DT == kKvF32 ? 1 : T::KS][3];
-  if constexpr (DT == kKvF32) {
-#pragma unroll
-    for (int i = 0; i < T::KL; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) qf[4 * i + j] = q_at(16 * i + 4 * g + j);
-  } else {
-    float x[T::KS][8];
-    float top = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < T::KS; ++ks)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[ks][j] = q_at(DT == kKvBF16 ? 32 * ks + 8 * g + j : 64 * (ks / 2) + 16 * g + 8 * (ks % 2) + j);
-        top = fmaxf(top, fabsf(x[ks][j]));
-      }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    // terms of values of about 1: the third one of a small query would fall
-    // below bf16's normal range
-    int e = (int)(bits_of(top) >> 23) - 127;
-    e = e < -126 || e > 126 ? 0 : e;
-    mult *= pow2f(e);
-#pragma unroll
-    for (int ks = 0; ks < T::KS; ++ks)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        __bf16 t[3];
-        split_bf16<3>(x[ks][j] * pow2f(-e), t);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) qt[ks][k][j] = t[k];
-      }
-  }
-
-  v4f acc[T::D];
-#pragma unroll
-  for (int d = 0; d < T::D; ++d) acc[d] = v4f{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.0f;
 
   const int row_bytes = p.pitch * T::ELEM;
   const int koff = c * row_bytes + 16 * g;
@@ -394,33 +429,36 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   const int vcol = c * T::D * T::ELEM < row_bytes ? c * T::D * T::ELEM : 0;
   const int voff = 4 * g * row_bytes + vcol;
 
-  // Pages of the tile's groups, stepping by the waves' tiles: index in the
-  // table and entry in the page.
-  const int step = W * KT, step_q = step / p.page_tokens, step_r = step - step_q * p.page_tokens;
-  int pidx[NSUB], poff[NSUB];
-#pragma unroll
-  for (int u = 0; u < NSUB; ++u) {
-    const int e = (t0 + wave) * KT + 16 * u;
-    pidx[u] = e / p.page_tokens, poff[u] = e - pidx[u] * p.page_tokens;
-  }
-  // pool rows of a tile's groups; a group without entries or page: -1
-  auto rows_of = [&](int t, int64_t (&row)[NSUB]) {
+  // Pages of this wave's tiles, 64 tiles at a time: lane i holds those of its
+  // i-th tile from `held` on. (A load of its own for every tile would be waited
+  // for at once, and with it, as loads return in order, all K and V loads.)
+  int page[NSUB], at[NSUB];
+  auto fetch = [&](int from) {
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
-      row[u] = -1;
-      if (t < t1 && t * KT + 16 * u < n) {
-        const int page = table[pidx[u]];
-        if (page >= 0 && page < p.num_pages)
-          row[u] = ((int64_t)page * p.kv_heads + h) * p.page_tokens + poff[u];
-      }
-      pidx[u] += step_q, poff[u] += step_r;
-      if (poff[u] >= p.page_tokens) poff[u] -= p.page_tokens, ++pidx[u];
+      const int t = from + W * lane, e = t * KT + 16 * u;
+      const int i = e / p.page_tokens;
+      page[u] = t < t1 && e < n ? table[i] : -1;
+      if (page[u] >= p.num_pages) page[u] = -1;
+      at[u] = e - i * p.page_tokens;
+    }
+  };
+  // pool rows of the groups of this wave's i-th tile; a group without entries
+  // or page: -1
+  auto rows_of = [&](int i, int64_t (&row)[NSUB]) {
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      const int pg = __builtin_amdgcn_readlane(page[u], i), off = __builtin_amdgcn_readlane(at[u], i);
+      row[u] = pg >= 0 ? ((int64_t)pg * p.kv_heads + h) * p.page_tokens + off : -1;
     }
   };
   u32x4 kr[NSUB][T::KL];
+  v4f ks[NSUB];
   auto load_k = [&](const int64_t (&row)[NSUB]) {
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
+      if constexpr (DT == kKvE4M3)
+        ks[u] = *reinterpret_cast<const v4f*>(p.ks + (row[u] < 0 ? 0 : row[u]) + 4 * g);
       const uint8_t* base = p.k + (row[u] < 0 ? 0 : row[u]) * row_bytes;
 #pragma unroll
       for (int i = 0; i < T::KL; ++i) {
@@ -431,59 +469,157 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
     }
   };
 
-  int64_t row[NSUB], next[NSUB];
-  rows_of(t0 + wave, row);
-  load_k(row);
-  for (int t = t0 + wave; t < t1; t += W) {
-    rows_of(t + W, next);
-    uint32_t vr[4 * NSUB][T::VW];
-    v4f ks[NSUB], vs[NSUB];
+  uint32_t vr[4 * NSUB][T::VW];
+  v4f vs[NSUB];
+  auto load_v = [&](const int64_t (&row)[NSUB]) {
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) {
       const int64_t r = row[u] < 0 ? 0 : row[u];
+      if constexpr (DT == kKvE4M3) vs[u] = *reinterpret_cast<const v4f*>(p.vs + r + 4 * g);
       const uint8_t* base = p.v + r * row_bytes;
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_words<T::VW>(vr[4 * u + i], base + voff + i * row_bytes);
-      if constexpr (DT == kKvE4M3) {
-        ks[u] = *reinterpret_cast<const v4f*>(p.ks + r + 4 * g);
-        vs[u] = *reinterpret_cast<const v4f*>(p.vs + r + 4 * g);
-      }
     }
-    // scores, the small terms apart from the large one
-    v4f x[NSUB];
+  };
+
+  int64_t row[NSUB], next[NSUB];
+  int i = 0;  // of the tile in the pages held
+  fetch(t0 + wave);
+  rows_of(0, row);
+  load_k(row);
+  load_v(row);
+  // queries: rows of heads in LDS with zeros around them, then this lane's part
+  // of the contraction; the bf16 terms in LDS too, alike for the four waves
+  const bool col_ok = c < cols;
+  const float slope =
+      GEN && a.alibi ? (float)(exp2(-8.0 * (double)(head0 + c + 1) / (double)p.heads) * kLog2e) : 0.0f;
+  float* qrows = reinterpret_cast<float*>(lds + QBYTES);
+  const float* q0 = a.q + (int64_t)b * a.q_stride + (int64_t)head0 * p.hd;
 #pragma unroll
-    for (int u = 0; u < NSUB; ++u) {
-      v4f big = {0.f, 0.f, 0.f, 0.f}, small = {0.f, 0.f, 0.f, 0.f};
-      if constexpr (DT == kKvF32) {
-#pragma unroll
-        for (int i = 0; i < T::KL; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v4f& to = i & 1 ? small : big;
-            to = __builtin_amdgcn_mfma_f32_16x16x4f32(float_of(kr[u][i][j]), qf[4 * i + j], to, 0, 0, 0);
-          }
+  for (int r = 0; r < (16 * HDP / 4 + 64 * W - 1) / (64 * W); ++r) {
+    const int item = threadIdx.x + 64 * W * r, col = item / (HDP / 4), d = 4 * (item % (HDP / 4));
+    v4f x = {0.f, 0.f, 0.f, 0.f};
+    if (col < cols) {
+      const float* from = q0 + col * p.hd + d;
+      if (part.vec_q) {
+        if (d < p.hd) x = *reinterpret_cast<const v4f*>(from);
       } else {
 #pragma unroll
-        for (int ks_ = 0; ks_ < T::KS; ++ks_) {
+        for (int j = 0; j < 4; ++j)
+          if (d + j < p.hd) x[j] = from[j];
+      }
+    }
+    if (col < 16) *reinterpret_cast<v4f*>(qrows + col * STRIDE + d) = x;
+  }
+  __syncthreads();
+  float mult = a.scale2;
+  float qf[DT == kKvF32 ? HDP / 4 : 1];
+  const float* qcol = qrows + c * STRIDE;
+  if constexpr (DT == kKvF32) {
+#pragma unroll
+    for (int i = 0; i < T::KL; ++i) {
+      const v4f x = *reinterpret_cast<const v4f*>(qcol + 16 * i + 4 * g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[4 * i + j] = x[j];
+    }
+    __syncthreads();
+  } else {
+    float top = 0.0f;
+    auto piece = [&](int step, int half) {
+      const int d = DT == kKvBF16 ? 32 * step + 8 * g : 64 * (step / 2) + 16 * g + 8 * (step % 2);
+      return *reinterpret_cast<const v4f*>(qcol + d + 4 * half);
+    };
+#pragma unroll
+    for (int j = 0; j < 2 * T::KS; ++j) {
+      const v4f x = piece(j / 2, j & 1);
+      top = fmaxf(fmaxf(fmaxf(top, fabsf(x[0])), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    // terms of values of about 1: the third one of a small query would fall
+    // below bf16's normal range
+    int e = (int)(bits_of(top) >> 23) - 127;
+    e = e < -126 || e > 126 ? 0 : e;
+    mult *= pow2f(e);
+    const float down = pow2f(-e);
+    for (int step = wave; step < T::KS; step += W) {
+      bf16x8 qt[3];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const v4f x = piece(step, half);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __bf16 t[3];
+          split_bf16<3>(x[j] * down, t);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) qt[k][4 * half + j] = t[k];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<bf16x8*>(lds + (step * 3 + k) * 1024 + 16 * lane) = qt[k];
+    }
+    __syncthreads();
+  }
+
+  v4f acc[T::D];
+#pragma unroll
+  for (int d = 0; d < T::D; ++d) acc[d] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f;
+
+  int qoff = 16 * lane;
+  for (int t = t0 + wave; t < t1; t += W) {
+    // (read from LDS again for every tile: kept in registers, the queries' terms
+    // cost a third of the waves)
+    asm volatile("" : "+v"(qoff));
+    if (++i == 64) {
+      i = 0;
+      fetch(t + W);
+    }
+    rows_of(i, next);
+    // scores, the small terms apart from the large one
+    v4f x[NSUB], small[NSUB];
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) x[u] = small[u] = v4f{0.f, 0.f, 0.f, 0.f};
+    if constexpr (DT == kKvF32) {
+#pragma unroll
+      for (int i = 0; i < T::KL; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v4f& to = i & 1 ? small[0] : x[0];
+          to = __builtin_amdgcn_mfma_f32_16x16x4f32(float_of(kr[0][i][j]), qf[4 * i + j], to, 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int step = 0; step < T::KS; ++step) {
+        bf16x8 qt[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          qt[k] = *reinterpret_cast<const bf16x8*>(lds + (step * 3 + k) * 1024 + qoff);
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
           bf16x8 k8;
           if constexpr (DT == kKvBF16) {
-            k8 = __builtin_bit_cast(bf16x8, kr[u][ks_]);
+            k8 = __builtin_bit_cast(bf16x8, kr[u][step]);
           } else {
-            const uint32_t w0 = kr[u][ks_ / 2][2 * (ks_ % 2)], w1 = kr[u][ks_ / 2][2 * (ks_ % 2) + 1];
+            const uint32_t w0 = kr[u][step / 2][2 * (step % 2)], w1 = kr[u][step / 2][2 * (step % 2) + 1];
             k8 = __builtin_bit_cast(bf16x8, u32x4{cvt_e4m3<false>(w0), cvt_e4m3<true>(w0),
                                                   cvt_e4m3<false>(w1), cvt_e4m3<true>(w1)});
           }
-          small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, qt[ks_][2], small, 0, 0, 0);
-          big = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, qt[ks_][0], big, 0, 0, 0);
-          small = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, qt[ks_][1], small, 0, 0, 0);
+          small[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, qt[2], small[u], 0, 0, 0);
+          x[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, qt[0], x[u], 0, 0, 0);
+          small[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8, qt[1], small[u], 0, 0, 0);
         }
       }
-      x[u] = (big + small) * mult;
+    }
+#pragma unroll
+    for (int u = 0; u < NSUB; ++u) {
+      x[u] = (x[u] + small[u]) * mult;
       if constexpr (DT == kKvE4M3) x[u] *= ks[u];
     }
     const bool rows_ok = row[0] >= 0 && row[NSUB - 1] >= 0;
-    const bool whole = rows_ok && (t + 1) * KT <= n && a.window <= 0;
-    if (a.alibi || a.window > 0) {
+    const bool whole = rows_ok && (t + 1) * KT <= n && (!GEN || a.window <= 0);
+    if (GEN && (a.alibi || a.window > 0)) {
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
         const int e = t * KT + 16 * u + 4 * g;
@@ -495,24 +631,19 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
         }
       }
     }
+    uint32_t unseen = 0;  // bit 4 u + i
     if (!whole) {
-      // entries that are not seen: weight 0, and no NaN of theirs times it
 #pragma unroll
       for (int u = 0; u < NSUB; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = t * KT + 16 * u + 4 * g + i;
           bool seen = row[u] >= 0 && e < n;
-          if (a.window > 0) seen = seen && qp - (pos ? pos[e < cap ? e : 0] : e) < a.window;
-          if (!seen) {
-            x[u][i] = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < T::VW; ++w) vr[4 * u + i][w] = 0;
-            if constexpr (DT == kKvE4M3) vs[u][i] = 0.0f;
-          }
+          if (GEN && a.window > 0) seen = seen && qp - (pos ? pos[e < cap ? e : 0] : e) < a.window;
+          if (!seen) x[u][i] = -INFINITY, unseen |= 1u << (4 * u + i);
         }
     }
-    if (part.scores && col_ok) {
+    if (GEN && part.scores && col_ok) {
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
         const int e = t * KT + 16 * u + 4 * g;
@@ -520,7 +651,9 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
           *reinterpret_cast<v4f*>(part.scores + ((size_t)b * p.heads + head0 + c) * cap + e) = x[u];
       }
     }
-    if (t + W < t1) load_k(next);
+    // (past the end: the pool's first rows; a branch around loads would make the
+    // compiler wait for all of them where it ends)
+    load_k(next);
 
     float top = x[0][0];
 #pragma unroll
@@ -545,8 +678,21 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
       for (int i = 0; i < 4; ++i) {
         w[4 * u + i] = __builtin_amdgcn_exp2f(x[u][i] - ref);
         l += w[4 * u + i];
-        if constexpr (DT == kKvE4M3) w[4 * u + i] *= vs[u][i];
       }
+    // weights of 0 have to meet values that are finite
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 4 * NSUB; ++j)
+        if (unseen >> j & 1) {
+#pragma unroll
+          for (int k = 0; k < T::VW; ++k) vr[j][k] = 0;
+          if constexpr (DT == kKvE4M3) vs[j / 4][j % 4] = 0.0f;
+        }
+    }
+    if constexpr (DT == kKvE4M3) {
+#pragma unroll
+      for (int j = 0; j < 4 * NSUB; ++j) w[j] *= vs[j / 4][j % 4];
+    }
     if constexpr (DT == kKvF32) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -582,98 +728,98 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v8, pt[k], acc[d], 0, 0, 0);
       }
     }
+    load_v(next);
 #pragma unroll
     for (int u = 0; u < NSUB; ++u) row[u] = next[u];
   }
 
-  // The waves' sums meet: waves 2 and 3 hand theirs to 0 and 1, then 1 to 0.
+  // The waves' sums meet in LDS (over the queries' terms), then every thread
+  // adds the four of its dims.
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  constexpr int STRIDE = HDP + 4;
-  __shared__ float ml[W][16][2];
-  __shared__ __attribute__((aligned(16))) float sums[2][16][STRIDE];
   if (g == 0) ml[wave][c][0] = m, ml[wave][c][1] = l;
   __syncthreads();
-  float M = -INFINITY, L = 0.0f;
+  float* sums = reinterpret_cast<float*>(lds);
+  if (col_ok) {
+    float M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < W; ++w) M = fmaxf(M, ml[w][c][0]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, ml[w][c][0]);
+    const float mine = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
+    float* to = sums + (wave * 16 + c) * STRIDE + 4 * g * T::D;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const float mw = ml[w][c][0];
-    L += ml[w][c][1] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < T::D; ++d) to[i * T::D + d] = acc[d][i] * mine;
   }
-  const float mine = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
-#pragma unroll
-  for (int d = 0; d < T::D; ++d) acc[d] *= mine;
-#pragma unroll
-  for (int half = 2; half >= 1; half /= 2) {
-    if (wave >= half && wave < 2 * half && col_ok) {
-#pragma unroll
-      for (int d = 0; d < T::D; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[wave - half][c][(4 * g + i) * T::D + d] = acc[d][i];
-    }
-    __syncthreads();
-    if (wave < half && col_ok) {
-#pragma unroll
-      for (int d = 0; d < T::D; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[d][i] += sums[wave][c][(4 * g + i) * T::D + d];
-    }
-    __syncthreads();
-  }
+  __syncthreads();
   if (part.info && place.index == 0 && blockIdx.y == 0 && threadIdx.x == 0)
-    part.info[2 * b] = place.slot, part.info[2 * b + 1] = place.parts;
-  if (place.parts == 1) {
-    if (wave != 0 || !col_ok) return;
-    const size_t head = (size_t)b * p.heads + head0 + c;
-    if (g == 0) {
+    part.info[b] = KvInfo{place.slot, place.parts, place.stride};
+  const bool one = place.parts == 1;
+  const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3, quads = pitch / 4;
+  const size_t me = one ? 0 : ((size_t)place.slot * gridDim.y + blockIdx.y) * most;
+  for (int item = threadIdx.x; item < cols * quads; item += 64 * W) {
+    const int col = item / quads, quad = item - col * quads;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, ml[w][col][0]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float mw = ml[w][col][0];
+      L += ml[w][col][1] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - M));
+    }
+    v4f o = *reinterpret_cast<const v4f*>(sums + col * STRIDE + 4 * quad);
+#pragma unroll
+    for (int w = 1; w < W; ++w)
+      o += *reinterpret_cast<const v4f*>(sums + (16 * w + col) * STRIDE + 4 * quad);
+    if (!one) {  // this part's sums, for k_kv_finish
+      if (quad == 0) part.ml[2 * (me + col)] = M, part.ml[2 * (me + col) + 1] = L;
+      *reinterpret_cast<v4f*>(part.out + (me + col) * pitch + 4 * quad) = o;
+      continue;
+    }
+    const size_t head = (size_t)b * p.heads + head0 + col;
+    if (quad == 0) {
       const float lse2 = L == 0.0f ? -INFINITY : M + __builtin_amdgcn_logf(L);
       if (a.lse) a.lse[head] = lse2 * kLn2;
       if (part.lse2) part.lse2[head] = lse2;
     }
-    float* out = a.out + (int64_t)b * a.out_stride + (int64_t)(head0 + c) * p.hd;
-    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+    o *= L == 0.0f ? 0.0f : 1.0f / L;
+    float* out = a.out + (int64_t)b * a.out_stride + (int64_t)(head0 + col) * p.hd + 4 * quad;
+    if (part.vec_out) {
+      *reinterpret_cast<v4f*>(out) = o;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int d = 0; d < T::D; ++d) {
-        const int dim = (4 * g + i) * T::D + d;
-        if (dim < p.hd) out[dim] = acc[d][i] * f;
-      }
-    return;
-  }
-
-  // more than one part: this one's sums, for k_kv_finish
-  const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3;
-  const size_t me = ((size_t)place.slot * gridDim.y + blockIdx.y) * most;
-  if (wave != 0 || !col_ok) return;
-  if (g == 0) part.ml[2 * (me + c)] = M, part.ml[2 * (me + c) + 1] = L;
-  float* to = part.out + (me + c) * pitch;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int d = 0; d < T::D; ++d) {
-      const int dim = (4 * g + i) * T::D + d;
-      if (dim < p.hd) to[dim] = acc[d][i];
+      for (int k = 0; k < 4; ++k)
+        if (4 * quad + k < p.hd) out[k] = o[k];
     }
+  }
+  if constexpr (RUNS) __syncthreads();  // (the sums are read)
+  } while (RUNS && kv_next<KT>(p, s, a, place));
+}
+
+template <class F>
+__device__ __forceinline__ float over_lanes(float x, int lane, F&& f) {
+  x = f(x, xor_lane<1>(x, lane));
+  x = f(x, xor_lane<2>(x, lane));
+  x = f(x, xor_lane<4>(x, lane));
+  x = f(x, xor_lane<8>(x, lane));
+  x = f(x, xor_lane<16>(x, lane));
+  return f(x, xor_lane<32>(x, lane));
 }
 
 // Reference and sum of a head's weights over its parts, in every lane of the
-// wave. ml: the first part's, `stride` floats from one to the next.
-__device__ __forceinline__ void join_sums(const float* ml, size_t stride, int parts, int lane,
-                                          float& top, float& sum) {
+// wave; at(i): where part i is.
+template <class F>
+__device__ __forceinline__ void join_sums(const float* ml, F&& at, int parts, int lane, float& top,
+                                          float& sum) {
   top = -INFINITY;
-  for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[i * stride]);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[2 * at(i)]);
+  top = over_lanes(top, lane, [](float x, float y) { return fmaxf(x, y); });
   sum = 0.0f;
   for (int i = lane; i < parts; i += 64) {
-    const float mi = ml[i * stride];
-    sum += ml[i * stride + 1] * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
+    const float mi = ml[2 * at(i)];
+    sum += ml[2 * at(i) + 1] * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  sum = over_lanes(sum, lane, [](float x, float y) { return x + y; });
 }
 
 // What follows the parts, for sequence blockIdx.z and K/V head blockIdx.y:
@@ -685,26 +831,27 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3;
   const size_t rows = (size_t)p.kv_heads * chunks;
-  const int slot = part.info[2 * b], parts = part.info[2 * b + 1];
-  // a head's first part, counted in heads, and the next part's
-  auto first_of = [&](int j) {
-    return ((size_t)slot * rows + (size_t)h * chunks + j / 16) * most + j % 16;
+  const KvInfo info = part.info[b];
+  const int parts = info.parts;
+  // part i of head j, counted in heads
+  auto of = [&](int i, int j) {
+    const size_t slot = (size_t)info.slot + (i ? 1 + (size_t)(i - 1) * info.stride : 0);
+    return (slot * rows + (size_t)h * chunks + j / 16) * most + j % 16;
   };
-  const size_t next = rows * most;
   if ((int)blockIdx.x < group) {
     if (parts == 1) return;  // written by the attention itself
     const int j = blockIdx.x;
-    const size_t base = first_of(j), head = (size_t)b * p.heads + (size_t)h * group + j;
+    const size_t head = (size_t)b * p.heads + (size_t)h * group + j;
     // four dims per thread, several teams of threads over the parts
     const int quads = pitch / 4, teams = 256 / quads;
     const int team = threadIdx.x / quads, quad = threadIdx.x - team * quads;
     float top, sum;
-    join_sums(part.ml + 2 * base, 2 * next, parts, lane, top, sum);
+    join_sums(part.ml, [&](int i) { return of(i, j); }, parts, lane, top, sum);
     v4f o = {0.f, 0.f, 0.f, 0.f};
     if (team < teams) {
 #pragma unroll 8
       for (int i = team; i < parts; i += teams) {
-        const size_t at = base + i * next;
+        const size_t at = of(i, j);
         const float mi = part.ml[2 * at];
         const v4f x = *reinterpret_cast<const v4f*>(part.out + at * pitch + 4 * quad);
         o += x * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
@@ -742,7 +889,7 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
         x = part.lse2[head + j0 + j];
       } else {
         float top, sum;
-        join_sums(part.ml + 2 * first_of(j0 + j), 2 * next, parts, lane, top, sum);
+        join_sums(part.ml, [&](int i) { return of(i, j0 + j); }, parts, lane, top, sum);
         x = sum == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
       }
       if (lane == 0) lse2[j] = x;
@@ -844,7 +991,7 @@ __device__ __forceinline__ void count_digits(const KvKeys<KPT>& keys, int step, 
 __device__ __forceinline__ uint32_t find_digit(const uint32_t* hist, int& need, int* red, int tid) {
   const int lane = tid & 63, wave = tid >> 6;
   const int c0 = (int)hist[kDigits - 1 - 2 * tid], c1 = (int)hist[kDigits - 2 - 2 * tid];
-  const int up = wave_scan(c0 + c1, lane);
+  const int up = wave_scan(c0 + c1);
   if (lane == 63) red[wave] = up;
   __syncthreads();
   int before = up - c0 - c1;
@@ -1047,7 +1194,7 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
       const int q = q0 + tid;
       KvCounts x;
       if (q < seg) x = counts[q];
-      const int eqs = x.eq_low + x.eq_high, up = wave_scan(eqs, lane);
+      const int eqs = x.eq_low + x.eq_high, up = wave_scan(eqs);
       int total, all;
       const int before = eq0 + waves_before(__builtin_amdgcn_readlane(up, 63), red, wave, lane, total) +
                          up - eqs;
@@ -1055,9 +1202,9 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
       low = q >= seg || low < 0 ? 0 : low < kSegment ? low : kSegment;
       const int hole = low - x.up_low - kept_at_cut(cut.ties, before, x.eq_low);
       const int tail = x.up_high + kept_at_cut(cut.ties, before + x.eq_low, x.eq_high);
-      waves_before((int)wave_sum(q < seg ? hole : 0), red, wave, lane, all);
+      waves_before(wave_sum(q < seg ? hole : 0), red, wave, lane, all);
       holes0 += all;
-      waves_before((int)wave_sum(q < seg ? tail : 0), red, wave, lane, all);
+      waves_before(wave_sum(q < seg ? tail : 0), red, wave, lane, all);
       tails0 += all;
       eq0 += total;
     }
@@ -1175,10 +1322,10 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
   }
   const int chunk_rows = kv_heads * kv_chunks(heads / kv_heads);
   const int most = heads / kv_heads < 16 ? heads / kv_heads : 16;
-  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows)) * chunk_rows * most;
+  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows, hd)) * chunk_rows * most;
   WV_TRY(c->part.alloc(slots * ((hd + 3) & ~3) * sizeof(float)));
   WV_TRY(c->part_ml.alloc(slots * 2 * sizeof(float)));
-  WV_TRY(c->info.alloc((size_t)max_seqs * 2 * sizeof(int32_t)));
+  WV_TRY(c->info.alloc((size_t)max_seqs * sizeof(KvInfo)));
   if (track && p.capacity() > kChooseOne) {
     const size_t choose_rows = (size_t)max_seqs * kv_heads;
     WV_TRY(c->choose_hist.alloc(choose_rows * 3 * kDigits * sizeof(uint32_t)));
@@ -1254,9 +1401,13 @@ Status launch_kv_read(const KvPool& p, const KvSeqs& s, int count, const int32_t
 }
 
 template <int DT>
-Status launch_attend(int hd, dim3 grid, const KvPool& p, const KvSeqs& s, const KvAttend& a,
+Status launch_attend(int hd, bool runs, dim3 grid, const KvPool& p, const KvSeqs& s, const KvAttend& a,
                      const KvPart& part, hipStream_t st) {
-#define WV_KV_HD(N) k_kv_attend<DT, N><<<grid, 256, 0, st>>>(p, s, a, part)
+  const bool gen = a.alibi || a.window > 0 || part.scores;
+#define WV_KV_HD(N)                                                                   \
+  (gen    ? k_kv_attend<DT, N, true, false><<<grid, 256, 0, st>>>(p, s, a, part)        \
+   : runs ? k_kv_attend<DT, N, false, true><<<grid, 256, 0, st>>>(p, s, a, part)        \
+          : k_kv_attend<DT, N, false, false><<<grid, 256, 0, st>>>(p, s, a, part))
   if constexpr (DT == kKvE4M3) {
     if (hd <= 64) WV_KV_HD(64);
     else if (hd <= 128) WV_KV_HD(128);
@@ -1279,21 +1430,27 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   const KvPool& p = c.pool;
   const int rows = p.kv_heads * kv_chunks(p.heads / p.kv_heads);
   KvPart part;
-  part.target = kv_target(rows);
+  part.target = kv_target(rows, p.hd);
   int64_t parts = kv_most_parts(s.nseq, part.target, p.capacity());
   if (parts <= s.nseq) part.target = 0, parts = s.nseq;
   part.out = c.part.as<float>();
   part.ml = c.part_ml.as<float>();
+  part.vec_q = p.hd % 4 == 0 && a.q_stride % 4 == 0 && (uintptr_t)a.q % 16 == 0;
+  part.vec_out = p.hd % 4 == 0 && a.out_stride % 4 == 0 && (uintptr_t)a.out % 16 == 0;
   const bool finish = part.target != 0 || s.weight;
-  if (finish) part.info = c.info.as<int32_t>();
+  if (finish) part.info = c.info.as<KvInfo>();
   if (s.weight) {
     part.scores = c.scores.as<float>();
     part.lse2 = c.lse2.as<float>();
   }
   const dim3 grid((unsigned)parts, (unsigned)rows);
-  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, grid, p, s, a, part, st)
-         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, grid, p, s, a, part, st)
-                              : launch_attend<kKvE4M3>(p.hd, grid, p, s, a, part, st));
+  // (with every sequence as long as it can be)
+  const int kt = p.dtype == kKvF32 ? 16 : 32;
+  const bool runs = s.nseq > 1 && part.target != 0 &&
+                    kv_runs((int64_t)s.nseq * ((p.capacity() + kt - 1) / kt), part.target, kt);
+  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, runs, grid, p, s, a, part, st)
+         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, runs, grid, p, s, a, part, st)
+                              : launch_attend<kKvE4M3>(p.hd, runs, grid, p, s, a, part, st));
   if (!finish) return Status::ok();
   const int most = (p.capacity() + 1023) / 1024;
   const int track = !s.weight ? 0 : most < 64 ? most : 64;
