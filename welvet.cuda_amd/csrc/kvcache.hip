@@ -811,14 +811,17 @@ __device__ __forceinline__ float over_lanes(float x, int lane, F&& f) {
 template <class F>
 __device__ __forceinline__ void join_sums(const float* ml, F&& at, int parts, int lane, float& top,
                                           float& sum) {
-  top = -INFINITY;
-  for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[2 * at(i)]);
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  v2f mine = {-INFINITY, 0.0f};  // of the first 64
+  if (lane < parts) mine = *reinterpret_cast<const v2f*>(ml + 2 * at(lane));
+  top = mine[0];
+  for (int i = lane + 64; i < parts; i += 64) top = fmaxf(top, ml[2 * at(i)]);
   top = over_lanes(top, lane, [](float x, float y) { return fmaxf(x, y); });
-  sum = 0.0f;
-  for (int i = lane; i < parts; i += 64) {
-    const float mi = ml[2 * at(i)];
-    sum += ml[2 * at(i) + 1] * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
-  }
+  auto part_sum = [&](float mi, float li) {
+    return li * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
+  };
+  sum = part_sum(mine[0], mine[1]);
+  for (int i = lane + 64; i < parts; i += 64) sum += part_sum(ml[2 * at(i)], ml[2 * at(i) + 1]);
   sum = over_lanes(sum, lane, [](float x, float y) { return x + y; });
 }
 
@@ -842,20 +845,32 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
     if (parts == 1) return;  // written by the attention itself
     const int j = blockIdx.x;
     const size_t head = (size_t)b * p.heads + (size_t)h * group + j;
-    // four dims per thread, several teams of threads over the parts
+    // four dims per thread, several teams of threads over the parts; the first
+    // eight parts of a team are on their way while the references are reduced
     const int quads = pitch / 4, teams = 256 / quads;
     const int team = threadIdx.x / quads, quad = threadIdx.x - team * quads;
+    constexpr int AHEAD = 8;
+    v4f x[AHEAD];
+    float mi[AHEAD];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * teams;
+        const size_t at = of(i < parts ? i : parts - 1, j);
+        mi[k] = part.ml[2 * at];
+        x[k] = *reinterpret_cast<const v4f*>(part.out + at * pitch + 4 * quad);
+      }
+    };
+    load(team);
     float top, sum;
     join_sums(part.ml, [&](int i) { return of(i, j); }, parts, lane, top, sum);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-    if (team < teams) {
-#pragma unroll 8
-      for (int i = team; i < parts; i += teams) {
-        const size_t at = of(i, j);
-        const float mi = part.ml[2 * at];
-        const v4f x = *reinterpret_cast<const v4f*>(part.out + at * pitch + 4 * quad);
-        o += x * (mi == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi - top));
-      }
+    for (int i0 = team; i0 < parts && team < teams; i0 += AHEAD * teams) {
+      if (i0 != team) load(i0);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * teams < parts)
+          o += x[k] * (mi[k] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mi[k] - top));
     }
     __shared__ v4f meet[256];
     meet[threadIdx.x] = o;
@@ -947,15 +962,29 @@ struct KvKeys {
     end = to;
     runs = (to - from + kChooseThreads - 1) / kChooseThreads;
     first = from + wave * runs * 64;
+    // (every load from a valid address and without a branch around it: the
+    // compiler would wait for each by itself; runs of no entries read the last)
+    float w[KPT];
+    int q[KPT];
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       const int e = entry(i, lane);
-      key[i] = 0;
-      if (i < runs && e < end) {
-        const int q = pos ? pos[e] : e;
-        key[i] = q < sinks || q >= late ? kKvKeyFirst : kv_weight_key(weight[e]);
-      }
+      q[i] = e < end ? e : end - 1;
+      w[i] = weight[q[i]];
     }
+    if (pos) {
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) q[i] = pos[q[i]];
+    }
+#pragma unroll
+    for (int i = 0; i < KPT; ++i)
+      key[i] = q[i] < sinks || q[i] >= late ? kKvKeyFirst : kv_weight_key(w[i]);
+  }
+  // How many of this wave's entries lie below the budget.
+  __device__ __forceinline__ int below(int budget) const {
+    int last = first + 64 * runs < end ? first + 64 * runs : end;
+    last = last < budget ? last : budget;
+    return last > first ? last - first : 0;
   }
   // f(i, e, in): for every run, with all lanes
   template <class F>
@@ -1040,16 +1069,14 @@ __device__ __forceinline__ KvCounts count_cut(const KvKeys<KPT>& keys, uint32_t 
   return c;
 }
 
-// Ranks the holes (hole; -1 elsewhere); WRITE: the kept entries below the
-// budget to src and those behind it to list. eq, holes, tails: how many come
-// before this wave.
-template <int KPT, bool WRITE>
+// Writes the kept entries below the budget to src, the holes' ranks in their
+// place (as -2 - rank), and the kept entries behind the budget to list. eq,
+// holes, tails: how many come before this wave.
+template <int KPT>
 __device__ __forceinline__ void place_kept(const KvKeys<KPT>& keys, const KvCut& cut, int budget,
                                            int eq, int holes, int tails, int32_t* src, int32_t* list,
-                                           int (&hole)[KPT], int lane) {
+                                           int lane) {
   const unsigned long long before = (1ull << lane) - 1;
-#pragma unroll
-  for (int i = 0; i < KPT; ++i) hole[i] = -1;
   keys.each(lane, [&](int i, int e, bool in) {
     const bool at = in && keys.key[i] == cut.least;
     const unsigned long long ats = __ballot(at);
@@ -1057,11 +1084,8 @@ __device__ __forceinline__ void place_kept(const KvKeys<KPT>& keys, const KvCut&
     eq += __popcll(ats);
     const bool low = in && e < budget;
     const unsigned long long hs = __ballot(low && !kept), ts = __ballot(in && !low && kept);
-    if (low && !kept) hole[i] = holes + __popcll(hs & before);
-    if constexpr (WRITE) {
-      if (low && kept) src[e] = e;
-      if (in && !low && kept) list[tails + __popcll(ts & before)] = e;
-    }
+    if (low) src[e] = kept ? e : -2 - (holes + __popcll(hs & before));
+    if (in && !low && kept) list[tails + __popcll(ts & before)] = e;
     holes += __popcll(hs);
     tails += __popcll(ts);
   });
@@ -1104,34 +1128,34 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvPool p, KvSeqs s
   const int eq = waves_before(c.eq_low + c.eq_high, red, wave, lane, total);
   const int kept_low = c.up_low + kept_at_cut(cut.ties, eq, c.eq_low);
   const int kept_high = c.up_high + kept_at_cut(cut.ties, eq + c.eq_low, c.eq_high);
-  int low = budget - keys.first;  // this wave's entries below the budget
-  const int mine = keys.end - keys.first < 64 * keys.runs ? keys.end - keys.first : 64 * keys.runs;
-  low = low < 0 ? 0 : low < mine ? low : mine < 0 ? 0 : mine;
+  const int low = keys.below(budget);
   const int holes = waves_before(low - kept_low, red, wave, lane, total);
   const int tails = waves_before(kept_high, red, wave, lane, total);
-  int hole[KPT];
-  place_kept<KPT, true>(keys, cut, budget, eq, holes, tails, src, list, hole, lane);
+  place_kept(keys, cut, budget, eq, holes, tails, src, list, lane);
   __syncthreads();
-  keys.each(lane, [&](int i, int e, bool) {
-    if (hole[i] >= 0) src[e] = list[hole[i]];
+  // (its own slots: every thread reads back what it wrote)
+  keys.each(lane, [&](int, int e, bool) {
+    const int at = e < budget ? src[e] : 0;
+    if (at < -1) src[e] = list[-2 - at];
   });
 }
 
 // Long sequences: every step of the above a launch, a workgroup per segment of
-// kSegment entries. The digits are counted in memory (zero between calls: the
-// last step clears them), the rest follows from the segments' counts.
-constexpr int kSegKeys = 16, kSegment = kSegKeys * kChooseThreads;
+// kSegment entries. The digits are counted in memory (zero between calls: step
+// 4 clears them), the ranks follow from the segments' counts. 2 x 8 rows of
+// 100003 entries: CHOOSEUS us, each launch SEGUS.
+constexpr int kSegKeys = 4, kSegment = kSegKeys * kChooseThreads;
 
 struct KvChooseLong {
   uint32_t* hist;    // [rows][3][kDigits]
-  KvCut* cut;        // [rows]
+  KvCut* cut;        // [rows][3]: after each digit
   KvCounts* counts;  // [rows][segments]
   int32_t* list;     // [rows][capacity / 2]
   int segments, budget, sinks, recent;
 };
 
 // STEP 0-2: count a digit; 3: count what is at and above the cut; 4: write
-// the kept entries and list those behind the budget; 5: fill the holes.
+// the kept entries and list those behind the budget.
 template <int STEP>
 __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvSeqs s, KvChooseLong c,
                                                                    int32_t* __restrict__ out) {
@@ -1152,12 +1176,17 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
   if (from >= n) return;
   KvKeys<kSegKeys> keys;
   keys.load(p, s, b, h, c.sinks, c.recent, n, from, to, wave, lane);
-  KvCut cut = {0u, budget};
   uint32_t* rows = c.hist + (size_t)row * 3 * kDigits;
-  if constexpr (STEP <= 3) {
-#pragma unroll
-    for (int step = 0; step < STEP; ++step)
-      cut.least |= find_digit(rows + step * kDigits, cut.ties, red, tid) << kShift[step];
+  KvCut* cuts = c.cut + (size_t)row * 3;
+  KvCut cut = {0u, budget};
+  if constexpr (STEP >= 1) {
+    if constexpr (STEP == 4) {
+      cut = cuts[2];
+    } else {
+      if constexpr (STEP > 1) cut = cuts[STEP - 2];
+      cut.least |= find_digit(rows + (STEP - 1) * kDigits, cut.ties, red, tid) << kShift[STEP - 1];
+      if (seg == 0 && tid == 0) cuts[STEP - 1] = cut;
+    }
   }
   if constexpr (STEP < 3) {
     hist[tid] = 0, hist[tid + kChooseThreads] = 0;
@@ -1168,7 +1197,6 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
       if (hist[i]) atomicAdd(rows + STEP * kDigits + i, hist[i]);
     return;
   }
-  if constexpr (STEP >= 4) cut = c.cut[row];
   KvCounts* counts = c.counts + (size_t)row * c.segments;
   const KvCounts w = count_cut(keys, cut.least, budget, lane);
   if constexpr (STEP == 3) {
@@ -1177,17 +1205,13 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
     waves_before(w.eq_high, red, wave, lane, all.eq_high);
     waves_before(w.up_low, red, wave, lane, all.up_low);
     waves_before(w.up_high, red, wave, lane, all.up_high);
-    if (tid == 0) {
-      counts[seg] = all;
-      if (seg == 0) c.cut[row] = cut;
-    }
-    return;
+    if (tid == 0) counts[seg] = all;
   }
-  if constexpr (STEP >= 4) {
-    if (STEP == 4)  // (the digits' counts are read no more)
-      for (int i = seg * kChooseThreads + tid; i < 3 * kDigits;
-           i += (n + kSegment - 1) / kSegment * kChooseThreads)
-        rows[i] = 0;
+  if constexpr (STEP == 4) {
+    // (the digits' counts are read no more)
+    for (int i = seg * kChooseThreads + tid; i < 3 * kDigits;
+         i += (n + kSegment - 1) / kSegment * kChooseThreads)
+      rows[i] = 0;
     // what lies in the segments before this one
     int eq0 = 0, holes0 = 0, tails0 = 0;
     for (int q0 = 0; q0 < seg; q0 += kChooseThreads) {
@@ -1212,20 +1236,20 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
     const int eq = eq0 + waves_before(w.eq_low + w.eq_high, red, wave, lane, total);
     const int kept_low = w.up_low + kept_at_cut(cut.ties, eq, w.eq_low);
     const int kept_high = w.up_high + kept_at_cut(cut.ties, eq + w.eq_low, w.eq_high);
-    int low = budget - keys.first;
-    const int mine = keys.end - keys.first < 64 * keys.runs ? keys.end - keys.first : 64 * keys.runs;
-    low = low < 0 ? 0 : low < mine ? low : mine < 0 ? 0 : mine;
+    const int low = keys.below(budget);
     const int holes = holes0 + waves_before(low - kept_low, red, wave, lane, total);
     const int tails = tails0 + waves_before(kept_high, red, wave, lane, total);
-    int32_t* list = c.list + (size_t)row * (cap / 2);
-    int hole[kSegKeys];
-    place_kept<kSegKeys, STEP == 4>(keys, cut, budget, eq, holes, tails, src, list, hole, lane);
-    if constexpr (STEP == 5) {
-      keys.each(lane, [&](int i, int e, bool) {
-        if (hole[i] >= 0) src[e] = list[hole[i]];
-      });
-    }
+    place_kept(keys, cut, budget, eq, holes, tails, src, c.list + (size_t)row * (cap / 2), lane);
   }
+}
+
+// The last step: the holes (-2 - rank) take the listed entries.
+__global__ __launch_bounds__(256) void k_kv_fill(int budget, int half, const int32_t* __restrict__ list,
+                                                 int32_t* __restrict__ out) {
+  const size_t row = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  const int at = j < budget ? out[row * budget + j] : 0;
+  if (at < -1) out[row * budget + j] = list[row * half - 2 - at];
 }
 
 // ---------------------------------------------------------------------------
@@ -1330,7 +1354,7 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
     const size_t choose_rows = (size_t)max_seqs * kv_heads;
     WV_TRY(c->choose_hist.alloc(choose_rows * 3 * kDigits * sizeof(uint32_t)));
     WV_HIP(hipMemsetAsync(c->choose_hist.p, 0, c->choose_hist.bytes, st));
-    WV_TRY(c->choose_cut.alloc(choose_rows * sizeof(KvCut)));
+    WV_TRY(c->choose_cut.alloc(choose_rows * 3 * sizeof(KvCut)));
     const size_t segments = (p.capacity() + kSegment - 1) / kSegment;
     WV_TRY(c->choose_counts.alloc(choose_rows * segments * sizeof(KvCounts)));
     WV_TRY(c->choose_list.alloc(choose_rows * (p.capacity() / 2) * sizeof(int32_t)));
@@ -1484,7 +1508,8 @@ Status kv_choose(const KvCache& c, const KvSeqs& s, int budget, int sinks, int r
     k_kv_choose_long<2><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
     k_kv_choose_long<3><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
     k_kv_choose_long<4><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
-    k_kv_choose_long<5><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
+    k_kv_fill<<<dim3((unsigned)blocks_of(budget), p.kv_heads, s.nseq), 256, 0, st>>>(budget, cap / 2,
+                                                                                   l.list, src);
   }
   return hip_status(hipGetLastError(), "k_kv_choose");
 }
