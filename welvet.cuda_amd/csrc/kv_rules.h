@@ -67,7 +67,7 @@ WV_HD int kv_chunks(int group) { return (group + 15) / 16; }
 
 // Waves per SIMD that the attention kernels' registers leave room for, by
 // head dims.
-WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 1; }
+WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 2; }
 
 // Workgroups (4 waves) per row (K/V head and chunk of query heads) that fill
 // 256 CUs once, and the tiles of `kt` entries that each takes of `tiles` (one

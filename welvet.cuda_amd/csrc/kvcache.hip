@@ -527,17 +527,8 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   }
   __syncthreads();
   float mult = a.scale2;
-  float qf[DT == kKvF32 ? HDP / 4 : 1];
   const float* qcol = qrows + c * STRIDE;
-  if constexpr (DT == kKvF32) {
-#pragma unroll
-    for (int i = 0; i < T::KL; ++i) {
-      const v4f x = *reinterpret_cast<const v4f*>(qcol + 16 * i + 4 * g);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) qf[4 * i + j] = x[j];
-    }
-    __syncthreads();
-  } else {
+  if constexpr (DT != kKvF32) {
     float top = 0.0f;
     auto piece = [&](int step, int half) {
       const int d = DT == kKvBF16 ? 32 * step + 8 * g : 64 * (step / 2) + 16 * g + 8 * (step % 2);
@@ -581,10 +572,10 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   for (int d = 0; d < T::D; ++d) acc[d] = v4f{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.0f;
 
-  int qoff = 16 * lane;
+  int qoff = DT == kKvF32 ? QBYTES + 4 * (c * STRIDE + 4 * g) : 16 * lane;
   for (int t = t0 + wave; t < t1; t += W) {
-    // (read from LDS again for every tile: kept in registers, the queries' terms
-    // cost a third of the waves)
+    // (the queries are read from LDS again for every tile: in registers they cost
+    // a third of the waves)
     asm volatile("" : "+v"(qoff));
     if (++i == 64) {
       i = 0;
@@ -597,12 +588,14 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
     for (int u = 0; u < NSUB; ++u) x[u] = small[u] = v4f{0.f, 0.f, 0.f, 0.f};
     if constexpr (DT == kKvF32) {
 #pragma unroll
-      for (int i = 0; i < T::KL; ++i)
+      for (int i = 0; i < T::KL; ++i) {
+        const v4f q = *reinterpret_cast<const v4f*>(lds + qoff + 64 * i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v4f& to = i & 1 ? small[0] : x[0];
-          to = __builtin_amdgcn_mfma_f32_16x16x4f32(float_of(kr[0][i][j]), qf[4 * i + j], to, 0, 0, 0);
+          to = __builtin_amdgcn_mfma_f32_16x16x4f32(float_of(kr[0][i][j]), q[j], to, 0, 0, 0);
         }
+      }
     } else {
 #pragma unroll
       for (int step = 0; step < T::KS; ++step) {
