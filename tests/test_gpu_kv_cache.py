@@ -194,6 +194,8 @@ def test_attend_over_long_caches(hip, oracle, dtype, lens, heads, kv, hd):
 @pytest.mark.parametrize("nseq,most,heads,kv,hd,dtype", [
     (70, 700, 2, 1, 64, km.E4M3), (130, 300, 20, 1, 32, km.BF16), (64, 900, 4, 4, 16, km.F32),
     (65, 2000, 1, 1, 64, km.BF16), (3, 4000, 34, 2, 64, km.BF16),
+    # (workgroups of one wave: 2048 rows of heads and more)
+    (300, 70, 8, 8, 64, km.BF16), (520, 40, 4, 4, 20, km.E4M3), (200, 400, 16, 16, 32, km.F32),
 ])
 def test_attend_over_many_unequal_sequences(hip, oracle, nseq, most, heads, kv, hd, dtype):
     """Sequences of none to many parts in one call, joined by kind."""

@@ -150,7 +150,7 @@ def test_parts_fit_the_grid_and_the_scratch(rules):
             lens = np.where(rng.random(nseq) < 0.1, lens, lens // 50)
         tiles = [-(-int(n) // kt) for n in lens]
         units = [max(1, t) for t in tiles]
-        target = rules.kv_check_target(rows, int(rng.integers(1, 257)))
+        target = rules.kv_check_target(rows, int(rng.integers(1, 257)), int(rng.integers(2)))
         step = rules.kv_check_part_tiles(sum(units), target, kt)
         most, slots = rules.kv_check_most_parts(nseq, target, cap), rules.kv_check_most_slots(target)
         if rules.kv_check_runs(sum(units), target, kt):

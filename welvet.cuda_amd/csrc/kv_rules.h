@@ -69,13 +69,20 @@ WV_HD int kv_chunks(int group) { return (group + 15) / 16; }
 // head dims.
 WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 2; }
 
-// Workgroups (4 waves) per row (K/V head and chunk of query heads) that fill
-// 256 CUs once, and the tiles of `kt` entries that each takes of `tiles` (one
-// at least per sequence): two for each wave, so that short sequences run side
-// by side, or an equal share. Shares of eight for each wave and more are runs
-// that go over the sequences' ends.
-WV_HD int kv_target(int kv_rows, int hd) {
-  const int n = 256 * kv_waves(hd) / kv_rows;
+// Workgroups of one wave instead of four: where the sequences' rows (K/V head
+// and chunk of query heads) fill a fifth of the GPU's waves by themselves. 1000
+// sequences of 8 to 64 entries, 32 heads over 8 of 128 in bf16, 8000 rows: 79.7
+// us with four waves, 42.2 with one; 256 of 38 to 300: 57.5 and 49.4; 64 of 64
+// to 512, 16 heads of 64, 1024 rows: 29.8 and 25.2. Fewer rows with more tiles
+// lose: 64 x 4096 E4M3 entries, 512 rows: 77.8 and 81.7.
+WV_HD bool kv_one_wave(int64_t rows, int hd) { return rows >= 200 * kv_waves(hd); }
+
+// Workgroups per row that fill 256 CUs once, and the tiles of `kt` entries
+// that each takes of `tiles` (one at least per sequence): two for each of four
+// waves, so that short sequences run side by side, or an equal share. Shares of
+// eight for each wave and more are runs that go over the sequences' ends.
+WV_HD int kv_target(int kv_rows, int hd, bool one_wave) {
+  const int n = 256 * kv_waves(hd) * (one_wave ? 4 : 1) / kv_rows;
   return n > 1 ? n : 1;
 }
 constexpr int kKvLeastEntries = 256;

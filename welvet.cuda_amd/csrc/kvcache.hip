@@ -412,12 +412,13 @@ __device__ __forceinline__ bool kv_next(const KvPool& p, const KvSeqs& s, const 
 }
 
 // GEN: ALiBi, windows, or scores for the running sums. RUNS: workgroups may take
-// runs over several sequences.
-template <int DT, int HDP, bool GEN, bool RUNS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kv_waves(HDP), 8)))
+// runs over several sequences. W waves per workgroup: 4, or 1 where sequences
+// and K/V heads are many (kv_one_wave).
+template <int DT, int HDP, bool GEN, bool RUNS, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kv_waves(HDP), 8)))
 void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   using T = KvShape<DT, HDP>;
-  constexpr int NSUB = T::NSUB, KT = 16 * NSUB, W = 4;
+  constexpr int NSUB = T::NSUB, KT = 16 * NSUB;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -853,26 +854,27 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
     const int j = blockIdx.x;
     const size_t head = (size_t)b * p.heads + (size_t)h * group + j;
     // four dims per thread, several teams of threads over the parts; the first
-    // eight parts of a team are on their way while the references are reduced
+    // four parts of a team are on their way while the references are reduced
     const int quads = pitch / 4, teams = 256 / quads;
     const int team = threadIdx.x / quads, quad = threadIdx.x - team * quads;
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 4;
     v4f x[AHEAD];
     float mi[AHEAD];
+    const int mine = team < teams ? parts : 0;
     auto load = [&](int i0) {
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int i = i0 + k * teams;
-        const size_t at = of(i < parts ? i : parts - 1, j);
+        const size_t at = of(i < parts ? i : i0, j);
         mi[k] = part.ml[2 * at];
         x[k] = *reinterpret_cast<const v4f*>(part.out + at * pitch + 4 * quad);
       }
     };
-    load(team);
+    if (team < mine) load(team);
     float top, sum;
     join_sums(part.ml, [&](int i) { return of(i, j); }, parts, lane, top, sum);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = team; i0 < parts && team < teams; i0 += AHEAD * teams) {
+    for (int i0 = team; i0 < mine; i0 += AHEAD * teams) {
       if (i0 != team) load(i0);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
@@ -1353,7 +1355,7 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
   }
   const int chunk_rows = kv_heads * kv_chunks(heads / kv_heads);
   const int most = heads / kv_heads < 16 ? heads / kv_heads : 16;
-  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows, hd)) * chunk_rows * most;
+  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows, hd, true)) * chunk_rows * most;
   WV_TRY(c->part.alloc(slots * ((hd + 3) & ~3) * sizeof(float)));
   WV_TRY(c->part_ml.alloc(slots * 2 * sizeof(float)));
   WV_TRY(c->info.alloc((size_t)max_seqs * sizeof(KvInfo)));
@@ -1432,13 +1434,15 @@ Status launch_kv_read(const KvPool& p, const KvSeqs& s, int count, const int32_t
 }
 
 template <int DT>
-Status launch_attend(int hd, bool runs, dim3 grid, const KvPool& p, const KvSeqs& s, const KvAttend& a,
+Status launch_attend(int hd, bool one, bool runs, dim3 grid, const KvPool& p, const KvSeqs& s, const KvAttend& a,
                      const KvPart& part, hipStream_t st) {
   const bool gen = a.alibi || a.window > 0 || part.scores;
-#define WV_KV_HD(N)                                                                   \
-  (gen    ? k_kv_attend<DT, N, true, false><<<grid, 256, 0, st>>>(p, s, a, part)        \
-   : runs ? k_kv_attend<DT, N, false, true><<<grid, 256, 0, st>>>(p, s, a, part)        \
-          : k_kv_attend<DT, N, false, false><<<grid, 256, 0, st>>>(p, s, a, part))
+#define WV_KV_HD(N)                                                                     \
+  (one && gen ? k_kv_attend<DT, N, true, false, 1><<<grid, 64, 0, st>>>(p, s, a, part)    \
+   : one      ? k_kv_attend<DT, N, false, false, 1><<<grid, 64, 0, st>>>(p, s, a, part)   \
+   : gen      ? k_kv_attend<DT, N, true, false, 4><<<grid, 256, 0, st>>>(p, s, a, part)   \
+   : runs     ? k_kv_attend<DT, N, false, true, 4><<<grid, 256, 0, st>>>(p, s, a, part)   \
+              : k_kv_attend<DT, N, false, false, 4><<<grid, 256, 0, st>>>(p, s, a, part))
   if constexpr (DT == kKvE4M3) {
     if (hd <= 64) WV_KV_HD(64);
     else if (hd <= 128) WV_KV_HD(128);
@@ -1461,7 +1465,8 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   const KvPool& p = c.pool;
   const int rows = p.kv_heads * kv_chunks(p.heads / p.kv_heads);
   KvPart part;
-  part.target = kv_target(rows, p.hd);
+  const bool one = kv_one_wave((int64_t)s.nseq * rows, p.hd);
+  part.target = kv_target(rows, p.hd, one);
   int64_t parts = kv_most_parts(s.nseq, part.target, p.capacity());
   if (parts <= s.nseq) part.target = 0, parts = s.nseq;
   part.out = c.part.as<float>();
@@ -1477,11 +1482,11 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   const dim3 grid((unsigned)parts, (unsigned)rows);
   // (with every sequence as long as it can be)
   const int kt = p.dtype == kKvF32 ? 16 : 32;
-  const bool runs = s.nseq > 1 && part.target != 0 &&
+  const bool runs = !one && s.nseq > 1 && part.target != 0 &&
                     kv_runs((int64_t)s.nseq * ((p.capacity() + kt - 1) / kt), part.target, kt);
-  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, runs, grid, p, s, a, part, st)
-         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, runs, grid, p, s, a, part, st)
-                              : launch_attend<kKvE4M3>(p.hd, runs, grid, p, s, a, part, st));
+  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, one, runs, grid, p, s, a, part, st)
+         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, one, runs, grid, p, s, a, part, st)
+                              : launch_attend<kKvE4M3>(p.hd, one, runs, grid, p, s, a, part, st));
   if (!finish) return Status::ok();
   const int most = (p.capacity() + 1023) / 1024;
   const int track = !s.weight ? 0 : most < 64 ? most : 64;
