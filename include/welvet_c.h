@@ -357,6 +357,30 @@ WELVET_API welvet_status welvet_kv_compact_device(welvet_kv_session* s, const we
 WELVET_API welvet_status welvet_kv_advance_device(welvet_kv_session* s, int32_t nseq, int32_t* lens,
                                                   int32_t* next_pos, const int32_t* counts,
                                                   int32_t add, int32_t cap, void* stream);
+/* Attention layers over a cache (mounted for the same heads), queued on
+ * `stream` (null: the MHA session's). The cache's rule on overlapping calls
+ * holds for both sessions.
+ * prefill: welvet_mha_execute_device of one sequence (a session mounted with
+ * batch 1), and K and V of its first `tokens` tokens (up to the mounted seq;
+ * the rows of x behind them are padding, which a causal layer's earlier tokens
+ * do not see) appended to the one sequence of seqs, which has to be empty:
+ * RoPE turns token i at position i.
+ * decode: one new token for each of nseq sequences (the batch of a session
+ * mounted with seq 1): x [nseq*d_model] is projected, Q and K turned at
+ * next_pos[b] (RoPE layers), K and V appended, pre [nseq*q_dim] is the
+ * attention over the sequence's entries and the new one, post [nseq*d_model]
+ * its O projection. The layer's window and ALiBi hold; its causal,
+ * bidirectional and prefix masks all leave the whole past. lens and next_pos
+ * stay as they are (welvet_kv_advance_device, once all layers have run). A
+ * sequence at its capacity keeps its entries: the token is not stored and
+ * attends to them alone. */
+WELVET_API welvet_status welvet_mha_prefill_device(welvet_mha_session* m, welvet_kv_session* s,
+                                                   const welvet_kv_seqs* seqs, int32_t tokens,
+                                                   const float* x, float* pre, float* post,
+                                                   void* stream);
+WELVET_API welvet_status welvet_mha_decode_device(welvet_mha_session* m, welvet_kv_session* s,
+                                                  const welvet_kv_seqs* seqs, const float* x,
+                                                  float* pre, float* post, void* stream);
 /* Model mount with a scale scheme: schemes 1-3 re-quantize each child's fp32
  * weights (the descriptor's Dense/SwiGLU/MHA W) with that scheme; 0 is
  * welvet_model_mount. */

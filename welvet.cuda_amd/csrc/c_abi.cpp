@@ -909,6 +909,46 @@ welvet_status welvet_kv_advance_device(welvet_kv_session* s, int32_t nseq, int32
   });
 }
 
+// Whether an attention layer and a cache have the same heads.
+static Status kv_matches(const wv::MHAConfig& c, const wv::KvPool& p) {
+  if (c.num_heads != p.heads || c.num_kv_heads != p.kv_heads || c.head_dim != p.hd)
+    return Status::err(wv::kInvalid, "mha: the cache was mounted for other heads");
+  return Status::ok();
+}
+
+welvet_status welvet_mha_prefill_device(welvet_mha_session* m, welvet_kv_session* s,
+                                        const welvet_kv_seqs* seqs, int32_t tokens, const float* x,
+                                        float* pre, float* post, void* stream) {
+  return guarded([&]() -> Status {
+    if (!m || !x || !pre || !post) return Status::err(wv::kInvalid, "mha prefill: invalid argument");
+    wv::KvSeqs q;
+    WV_TRY(kv_seqs(s, seqs, &q));
+    WV_TRY(kv_matches(m->layer.cfg, s->cache.pool));
+    if (m->batch != 1 || q.nseq != 1)
+      return Status::err(wv::kInvalid, "mha prefill: one sequence, in a session mounted with batch 1");
+    if (tokens < 0 || tokens > m->seq || tokens > s->cache.pool.capacity())
+      return Status::err(wv::kInvalid, "mha prefill: tokens outside the mounted seq or the capacity");
+    return wv::mha_prefill(m->layer, s->cache, q, m->seq, tokens, x, pre, post, &m->ws,
+                           pick(stream, m->stream.s));
+  });
+}
+
+welvet_status welvet_mha_decode_device(welvet_mha_session* m, welvet_kv_session* s,
+                                       const welvet_kv_seqs* seqs, const float* x, float* pre,
+                                       float* post, void* stream) {
+  return guarded([&]() -> Status {
+    if (!m || !x || !pre || !post) return Status::err(wv::kInvalid, "mha decode: invalid argument");
+    wv::KvSeqs q;
+    WV_TRY(kv_seqs(s, seqs, &q));
+    WV_TRY(kv_matches(m->layer.cfg, s->cache.pool));
+    if (m->seq != 1 || q.nseq != m->batch)
+      return Status::err(wv::kInvalid, "mha decode: nseq must be the batch of a session mounted with seq 1");
+    if (q.weight && !s->cache.track)
+      return Status::err(wv::kInvalid, "mha decode: running sums need a cache mounted with WELVET_KV_TRACK");
+    return wv::mha_decode(m->layer, s->cache, q, x, pre, post, &m->ws, pick(stream, m->stream.s));
+  });
+}
+
 // ---------------------------------------------------------------- model ----
 struct welvet_model_session {
   std::mutex mu;

@@ -54,6 +54,10 @@ struct KvRows {
   int64_t k_stride = 0, v_stride = 0;
 };
 Status launch_kv_append(const KvPool& p, const KvSeqs& s, const KvRows& r, hipStream_t st);
+// RoPE of one token per sequence at next_pos (lens without it): the pairs (d, d
+// + hd / 2) of every head of q and k rows turned by next_pos / theta^(2 d / hd).
+Status launch_kv_rope(float* q, float* k, int heads, int kv_heads, int hd, int q_stride,
+                      int kv_stride, double theta, const KvPool& p, const KvSeqs& s, hipStream_t st);
 Status launch_kv_read(const KvPool& p, const KvSeqs& s, int count, const int32_t* first,
                       const int32_t* counts, float* k, float* v, hipStream_t st);
 

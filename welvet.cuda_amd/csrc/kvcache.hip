@@ -260,8 +260,9 @@ struct KvShape {
 template <int KT>
 __device__ __forceinline__ void kv_sequence(const KvPool& p, const KvSeqs& s, const KvAttend& a, int b,
                                             int& n, int& qp, int& first, int& tiles) {
-  n = kv_entries(s.lens[b], a.tail, p.capacity());
-  qp = (s.next_pos ? s.next_pos[b] : n - a.tail) + a.tail - 1;
+  const int len = s.lens[b];
+  n = kv_entries(len, a.tail, p.capacity());
+  qp = (s.next_pos ? s.next_pos[b] : kv_entries(len, 0, p.capacity())) + a.tail - 1;
   first = kv_first_tile(n, qp, s.pos == nullptr ? a.window : 0, KT);
   tiles = (n + KT - 1) / KT - first;
 }
@@ -1317,6 +1318,31 @@ __global__ __launch_bounds__(256) void k_kv_compact(KvPool p, KvSeqs s, int budg
   }
 }
 
+// ---------------------------------------------------------------------------
+// RoPE of one token per sequence (launch_kv_rope), in f64 as the attention
+// layers' own (k_rope): a workgroup per sequence forms the angles once for all
+// heads.
+__global__ __launch_bounds__(256) void k_kv_rope(float* __restrict__ q, float* __restrict__ k,
+                                                 int heads, int kv_heads, int hd, int q_stride,
+                                                 int kv_stride, double theta, KvPool p, KvSeqs s) {
+  const int b = blockIdx.x, half = hd / 2;
+  __shared__ double cs[kKvMaxHd / 2][2];
+  const int t = s.next_pos ? s.next_pos[b] : kv_entries(s.lens[b], 0, p.capacity());
+  for (int d = threadIdx.x; d < half; d += 256) {
+    const double ang = (double)t / pow(theta, (double)(2 * d) / (double)hd);
+    cs[d][0] = cos(ang), cs[d][1] = sin(ang);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (heads + kv_heads) * half; i += 256) {
+    const int h = i / half, d = i - h * half;
+    float* row = h < heads ? q + (size_t)b * q_stride + (size_t)h * hd
+                           : k + (size_t)b * kv_stride + (size_t)(h - heads) * hd;
+    const double c = cs[d][0], n = cs[d][1], a0 = row[d], a1 = row[d + half];
+    row[d] = (float)(a0 * c - a1 * n);
+    row[d + half] = (float)(a0 * n + a1 * c);
+  }
+}
+
 __global__ void k_kv_advance(int nseq, int32_t* lens, int32_t* next_pos,
                              const int32_t* __restrict__ counts, int add, int cap) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
@@ -1537,6 +1563,14 @@ Status launch_kv_compact(const KvPool& p, const KvSeqs& s, int budget, const int
   else if (pieces <= 32) k_kv_compact<32><<<grid, 256, 0, st>>>(p, s, budget, src);
   else k_kv_compact<64><<<grid, 256, 0, st>>>(p, s, budget, src);
   return hip_status(hipGetLastError(), "k_kv_compact");
+}
+
+Status launch_kv_rope(float* q, float* k, int heads, int kv_heads, int hd, int q_stride,
+                      int kv_stride, double theta, const KvPool& p, const KvSeqs& s, hipStream_t st) {
+  if (s.nseq == 0 || hd < 2) return Status::ok();
+  if (hd > kKvMaxHd) return Status::err(kUnsupported, "kv rope: head_dim above 256");
+  k_kv_rope<<<s.nseq, 256, 0, st>>>(q, k, heads, kv_heads, hd, q_stride, kv_stride, theta, p, s);
+  return hip_status(hipGetLastError(), "k_kv_rope");
 }
 
 Status launch_kv_advance(int nseq, int32_t* lens, int32_t* next_pos, const int32_t* counts, int add,

@@ -1061,6 +1061,53 @@ Status mha_prepare(const MHALayer& L, int batch, int seq, Workspace* ws) {
   return ensure_split(ws, mha_split_bytes(L, batch * seq));
 }
 
+MHARows mha_rows(const MHALayer& L, int T, const Workspace& ws) {
+  const MHAConfig& c = L.cfg;
+  MHARows r;
+  // joined: a token's Q, K and V follow each other in one row
+  const bool joined = L.qkv.out != 0;
+  r.q = ws.a.as<float>();
+  r.k = r.q + (joined ? 1 : (size_t)T) * c.q_dim();
+  r.v = r.k + (joined ? 1 : (size_t)T) * c.kv_dim();
+  r.q_stride = joined ? L.qkv.out : c.q_dim();
+  r.kv_stride = joined ? L.qkv.out : c.kv_dim();
+  return r;
+}
+
+// The Q, K and V rows of T tokens in ws->a (mha_rows); with rope_epi, Q and K
+// turned at positions 0 .. T - 1 by the products' epilogues.
+static Status mha_project(const MHALayer& L, int T, const float* x, bool rope_epi, Workspace* ws,
+                          hipStream_t st) {
+  const MHAConfig& c = L.cfg;
+  const MHARows r = mha_rows(L, T, *ws);
+  const bool joined = L.qkv.out != 0;
+  if (joined && uses_split(T)) {
+    WV_TRY(ensure_split(ws, mha_split_bytes(L, T)));
+    // (read by the attention kernel next: kept in the caches)
+    return dense_forward_split(L.qkv, T, x, false, ws, r.q, nullptr, st,
+                               rope_epi ? ws->c.as<const double>() : nullptr,
+                               rope_epi ? c.head_dim : 0, true, nullptr, c.q_dim() + c.kv_dim());
+  }
+  if (joined) return dense_forward(L.qkv, T, x, r.q, nullptr, ws, st);
+  if (uses_split(T)) {
+    // Q, K and V read the same activations: above 32 rows they are split
+    // once (up to 32 rows each GEMM kernel splits its own K range)
+    WV_TRY(ensure_split(ws, mha_split_bytes(L, T)));
+    const bool once = mxg_block_m(T) > 16;
+    const double* tab = rope_epi ? ws->c.as<const double>() : nullptr;
+    const int rhd = rope_epi ? c.head_dim : 0;
+    if (once)
+      WV_TRY(launch_split(x, c.d_model, T, c.d_model, L.q.dev.kpad, split_buf(ws), st, L.q.terms));
+    // (Q, K and V are read by the attention kernel next: kept in the caches)
+    WV_TRY(dense_forward_split(L.q, T, x, once, ws, r.q, nullptr, st, tab, rhd, true));
+    WV_TRY(dense_forward_split(L.k, T, x, once, ws, r.k, nullptr, st, tab, rhd, true));
+    return dense_forward_split(L.v, T, x, once, ws, r.v, nullptr, st, nullptr, 0, true);
+  }
+  WV_TRY(dense_forward(L.q, T, x, r.q, nullptr, ws, st));
+  WV_TRY(dense_forward(L.k, T, x, r.k, nullptr, ws, st));
+  return dense_forward(L.v, T, x, r.v, nullptr, ws, st);
+}
+
 Status mha_forward(const MHALayer& L, int batch, int seq, const float* x, float* attn, float* y,
                    Workspace* ws, hipStream_t st) {
   const MHAConfig& c = L.cfg;
@@ -1070,11 +1117,7 @@ Status mha_forward(const MHALayer& L, int batch, int seq, const float* x, float*
   const size_t need = mha_workspace_bytes(L, batch, seq);
   if (ws->a.bytes < need) WV_TRY(ws->a.alloc(need));
   const int T = batch * seq;
-  float* qb = ws->a.as<float>();
-  // joined: a token's Q, K and V follow each other in one row
   const bool joined = L.qkv.out != 0;
-  float* kb = qb + (joined ? 1 : (size_t)T) * c.q_dim();
-  float* vb = kb + (joined ? 1 : (size_t)T) * c.kv_dim();
   // RoPE in the Q and K GEMM epilogues (large tiles): the attention kernel
   // then reads rotated rows
   const bool rope = mha_rope(c);
@@ -1087,36 +1130,11 @@ Status mha_forward(const MHALayer& L, int batch, int seq, const float* x, float*
                         // followed by k_rope
                         !(joined && mxg_part_bytes(T, L.qkv.dev.kpad, L.qkv.out, 1) > 0);
   if (rope) WV_TRY(ensure_rope_table(L, T, ws, st));
-  if (joined && uses_split(T)) {
-    WV_TRY(ensure_split(ws, mha_split_bytes(L, T)));
-    // (read by the attention kernel next: kept in the caches)
-    WV_TRY(dense_forward_split(L.qkv, T, x, false, ws, qb, nullptr, st,
-                               rope_epi ? ws->c.as<const double>() : nullptr,
-                               rope_epi ? c.head_dim : 0, true, nullptr, c.q_dim() + c.kv_dim()));
-  } else if (joined) {
-    WV_TRY(dense_forward(L.qkv, T, x, qb, nullptr, ws, st));
-  } else if (uses_split(T)) {
-    // Q, K and V read the same activations: above 32 rows they are split
-    // once (up to 32 rows each GEMM kernel splits its own K range)
-    WV_TRY(ensure_split(ws, mha_split_bytes(L, T)));
-    const bool once = mxg_block_m(T) > 16;
-    const double* tab = rope_epi ? ws->c.as<const double>() : nullptr;
-    const int rhd = rope_epi ? c.head_dim : 0;
-    if (once)
-      WV_TRY(launch_split(x, c.d_model, T, c.d_model, L.q.dev.kpad, split_buf(ws), st, L.q.terms));
-    // (Q, K and V are read by the attention kernel next: kept in the caches)
-    WV_TRY(dense_forward_split(L.q, T, x, once, ws, qb, nullptr, st, tab, rhd, true));
-    WV_TRY(dense_forward_split(L.k, T, x, once, ws, kb, nullptr, st, tab, rhd, true));
-    WV_TRY(dense_forward_split(L.v, T, x, once, ws, vb, nullptr, st, nullptr, 0, true));
-  } else {
-    WV_TRY(dense_forward(L.q, T, x, qb, nullptr, ws, st));
-    WV_TRY(dense_forward(L.k, T, x, kb, nullptr, ws, st));
-    WV_TRY(dense_forward(L.v, T, x, vb, nullptr, ws, st));
-  }
+  WV_TRY(mha_project(L, T, x, rope_epi, ws, st));
+  const MHARows r = mha_rows(L, T, *ws);
   AttnArgs a;
-  a.q = qb, a.k = kb, a.v = vb, a.out = attn;
-  a.q_stride = joined ? L.qkv.out : c.q_dim();
-  a.kv_stride = joined ? L.qkv.out : c.kv_dim();
+  a.q = r.q, a.k = r.k, a.v = r.v, a.out = attn;
+  a.q_stride = r.q_stride, a.kv_stride = r.kv_stride;
   a.tokens = T, a.seq = seq, a.heads = c.num_heads, a.kv_heads = c.num_kv_heads;
   a.hd = c.head_dim, a.msl = c.max_seq_len;
   a.mask = c.mask, a.window = c.window, a.prefix_len = c.prefix_len;
@@ -1141,6 +1159,44 @@ Status mha_forward(const MHALayer& L, int batch, int seq, const float* x, float*
     return dense_forward_split(L.o, T, attn, true, ws, y, nullptr, st);
   }
   WV_TRY(launch_attention(a, st));
+  return dense_forward(L.o, T, attn, y, nullptr, ws, st);
+}
+
+Status mha_prefill(const MHALayer& L, const KvCache& cache, const KvSeqs& seqs, int seq, int tokens,
+                   const float* x, float* attn, float* y, Workspace* ws, hipStream_t st) {
+  WV_TRY(mha_forward(L, 1, seq, x, attn, y, ws, st));
+  // K as the attention read it: turned at its position
+  const MHARows r = mha_rows(L, seq, *ws);
+  KvRows rows;
+  rows.rows = tokens;
+  rows.k = r.k, rows.v = r.v, rows.k_stride = rows.v_stride = r.kv_stride;
+  return launch_kv_append(cache.pool, seqs, rows, st);
+}
+
+Status mha_decode(const MHALayer& L, const KvCache& cache, const KvSeqs& seqs, const float* x,
+                  float* attn, float* y, Workspace* ws, hipStream_t st) {
+  const MHAConfig& c = L.cfg;
+  const int T = seqs.nseq;
+  if (T == 0) return Status::ok();
+  if (c.softmax == 1) return Status::err(kUnsupported, "mha decode: sigmoid attention has no cached form");
+  WV_TRY(mha_project(L, T, x, false, ws, st));
+  const MHARows r = mha_rows(L, T, *ws);
+  if (mha_rope(c))
+    WV_TRY(launch_kv_rope(r.q, r.k, c.num_heads, c.num_kv_heads, c.head_dim, r.q_stride, r.kv_stride,
+                          c.rope_theta, cache.pool, seqs, st));
+  KvRows rows;
+  rows.rows = 1;
+  rows.k = r.k, rows.v = r.v, rows.k_stride = rows.v_stride = r.kv_stride;
+  WV_TRY(launch_kv_append(cache.pool, seqs, rows, st));
+  KvAttend a;
+  a.q = r.q, a.q_stride = r.q_stride, a.out = attn, a.out_stride = c.q_dim();
+  a.tail = 1;
+  // (all entries lie before the token: the other masks leave them all)
+  a.window = c.mask == 3 ? (c.window > 0 ? c.window : c.max_seq_len) : 0;
+  a.alibi = (c.pos == 2 || c.pos == 3) ? 1 : 0;
+  const double scale = c.scale_override > 0 ? c.scale_override : 1.0 / std::sqrt((double)c.head_dim);
+  a.scale2 = (float)(scale * 1.4426950408889634);
+  WV_TRY(kv_attend(cache, seqs, a, st));
   return dense_forward(L.o, T, attn, y, nullptr, ws, st);
 }
 

@@ -6,6 +6,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "kvcache.h"
 #include "runtime.h"
 
 namespace wv {
@@ -274,6 +275,24 @@ Status mha_build(const MHAConfig& cfg, int dtype, int scheme, const float* Q, co
 Status mha_forward(const MHALayer& L, int batch, int seq, const float* x, float* attn, float* y,
                    Workspace* ws, hipStream_t st);
 size_t mha_workspace_bytes(const MHALayer& L, int batch, int seq);
+// Q, K and V rows of a forward's T tokens in its workspace (floats from a row
+// to the next one).
+struct MHARows {
+  float* q = nullptr;
+  float* k = nullptr;
+  float* v = nullptr;
+  int q_stride = 0, kv_stride = 0;
+};
+MHARows mha_rows(const MHALayer& L, int T, const Workspace& ws);
+// mha_forward of one sequence of `seq` tokens, then K and V of the first
+// `tokens` of them appended to seqs (one empty sequence).
+Status mha_prefill(const MHALayer& L, const KvCache& cache, const KvSeqs& seqs, int seq, int tokens,
+                   const float* x, float* attn, float* y, Workspace* ws, hipStream_t st);
+// One new token per sequence: x [nseq][d], projected, Q and K turned at
+// next_pos, K and V appended, attn [nseq][q_dim] the attention over the cache
+// with them, y [nseq][d]. ws is sized for nseq tokens (mha_prepare).
+Status mha_decode(const MHALayer& L, const KvCache& cache, const KvSeqs& seqs, const float* x,
+                  float* attn, float* y, Workspace* ws, hipStream_t st);
 // Sizes the workspace for (batch, seq) ahead of forward calls.
 Status mha_prepare(const MHALayer& L, int batch, int seq, Workspace* ws);
 

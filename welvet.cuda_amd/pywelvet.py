@@ -154,6 +154,8 @@ def lib():
     _sig(L, "welvet_kv_choose_device", Status, [_vp, seqs, _i32, _i32, _i32, _vp, _vp])
     _sig(L, "welvet_kv_compact_device", Status, [_vp, seqs, _i32, _vp, _vp])
     _sig(L, "welvet_kv_advance_device", Status, [_vp, _i32, _vp, _vp, _vp, _i32, _i32, _vp])
+    _sig(L, "welvet_mha_prefill_device", Status, [_vp, _vp, seqs, _i32, _vp, _vp, _vp, _vp])
+    _sig(L, "welvet_mha_decode_device", Status, [_vp, _vp, seqs, _vp, _vp, _vp, _vp])
     _sig(L, "welvet_model_abi_version", _i32, [])
     _sig(L, "welvet_model_mount", Status, [_u8p, _sz, ctypes.POINTER(_vp)])
     _sig(L, "welvet_model_mount_q", Status, [_u8p, _sz, _i32, ctypes.POINTER(_vp)])
@@ -585,6 +587,14 @@ class MHASession:
     def execute_device(self, x, pre, post, stream=None):
         check(lib().welvet_mha_execute_device(self.h, _vp(x), _vp(pre), _vp(post),
                                               _vp(stream) if stream else None))
+
+    def prefill(self, cache, seqs, tokens, x, pre, post, stream=None):
+        check(lib().welvet_mha_prefill_device(self.h, cache.h, ctypes.byref(seqs), tokens, x, pre,
+                                              post, stream))
+
+    def decode(self, cache, seqs, x, pre, post, stream=None):
+        check(lib().welvet_mha_decode_device(self.h, cache.h, ctypes.byref(seqs), x, pre, post,
+                                             stream))
 
     def close(self):
         if self.h:
