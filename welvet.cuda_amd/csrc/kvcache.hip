@@ -1025,6 +1025,14 @@ __device__ __forceinline__ void count_digits(const KvKeys<KPT>& keys, int step, 
   });
 }
 
+// Sum of the 16 waves' values before this one's; total: of all.
+__device__ __forceinline__ int sum_before(const int* red, int wave, int lane, int& total) {
+  static_assert(kChooseWaves == 16, "a row of 16 lanes holds the waves' values");
+  const int up = wave_scan(red[lane & 15]);
+  total = __builtin_amdgcn_readlane(up, 15);
+  return wave ? __builtin_amdgcn_readlane(up, wave ? wave - 1 : 0) : 0;
+}
+
 // The digit of the need-th key from the top of hist (every thread calls);
 // need becomes its rank among the keys of that digit.
 __device__ __forceinline__ uint32_t find_digit(const uint32_t* hist, int& need, int* red, int tid) {
@@ -1033,8 +1041,8 @@ __device__ __forceinline__ uint32_t find_digit(const uint32_t* hist, int& need, 
   const int up = wave_scan(c0 + c1);
   if (lane == 63) red[wave] = up;
   __syncthreads();
-  int before = up - c0 - c1;
-  for (int w = 0; w < kChooseWaves; ++w) before += w < wave ? red[w] : 0;
+  int all;
+  const int before = up - c0 - c1 + sum_before(red, wave, lane, all);
   if (before < need && need <= before + c0 + c1) {
     const bool second = need > before + c0;
     red[kChooseWaves] = kDigits - 1 - 2 * tid - (second ? 1 : 0);
@@ -1052,13 +1060,7 @@ __device__ __forceinline__ int waves_before(int x, int* red, int wave, int lane,
   __syncthreads();
   if (lane == 0) red[wave] = x;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < kChooseWaves; ++w) {
-    before += w < wave ? red[w] : 0;
-    total += red[w];
-  }
-  return before;
+  return sum_before(red, wave, lane, total);
 }
 
 // Entries at the cut, and above it, of a wave: below the budget and behind it.
