@@ -709,13 +709,19 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
         for (int d = 0; d < T::D; ++d)
           acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(float_of(vr[i][d]), w[i], acc[d], 0, 0, 0);
     } else {
+      // three terms of 8 bits each by cutting: they hold a weight's 24 exactly
       bf16x8 pt[3];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        __bf16 t3[3];
-        split_bf16<3>(w[j], t3);
+      for (int k = 0; k < 3; ++k) {
+        u32x4 f;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) pt[k][j] = t3[k];
+        for (int j = 0; j < 4; ++j)
+          f[j] = __builtin_amdgcn_perm(bits_of(w[2 * j + 1]), bits_of(w[2 * j]), 0x07060302u);
+        pt[k] = __builtin_bit_cast(bf16x8, f);
+        if (k < 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] -= float_of(bits_of(w[j]) & 0xFFFF0000u);
+        }
       }
 #pragma unroll
       for (int d = 0; d < T::D; ++d) {
