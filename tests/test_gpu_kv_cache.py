@@ -196,6 +196,9 @@ def test_attend_over_long_caches(hip, oracle, dtype, lens, heads, kv, hd):
     (65, 2000, 1, 1, 64, km.BF16), (3, 4000, 34, 2, 64, km.BF16),
     # (workgroups of one wave: 2048 rows of heads and more)
     (300, 70, 8, 8, 64, km.BF16), (520, 40, 4, 4, 20, km.E4M3), (200, 400, 16, 16, 32, km.F32),
+    # (the same with several query heads to a K/V head, up to all columns of a tile)
+    (300, 40, 12, 4, 64, km.BF16), (330, 35, 20, 1, 128, km.BF16), (110, 50, 64, 4, 256, km.BF16),
+    (200, 60, 16, 4, 80, km.E4M3), (450, 33, 5, 1, 250, km.E4M3), (210, 45, 48, 3, 128, km.F32),
 ])
 def test_attend_over_many_unequal_sequences(hip, oracle, nseq, most, heads, kv, hd, dtype):
     """Sequences of none to many parts in one call, joined by kind."""

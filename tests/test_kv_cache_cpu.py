@@ -46,6 +46,8 @@ def mount(dtype=3, pages=4, page=16, heads=4, kv=2, hd=64, seqs=2, max_pages=2, 
     (dict(heads=0), 1), (dict(kv=0), 1), (dict(heads=5), 1), (dict(hd=0), 1), (dict(hd=-4), 1),
     (dict(hd=257), 2), (dict(seqs=0), 1), (dict(seqs=65536), 1), (dict(max_pages=0), 1),
     (dict(max_pages=1 << 27), 1), (dict(max_pages=2 ** 31 - 1, page=2 ** 31 - 16), 1),
+    (dict(pages=2 ** 31 - 1, heads=60000, kv=60000, page=2 ** 20), 1),  # rows past 64 bits of bytes
+    (dict(pages=1, heads=65535, kv=1, seqs=65535, max_pages=2 ** 26, flags=1), 1),
     (dict(flags=2), 1), (dict(dtype=0), 2), (dict(dtype=2), 2), (dict(dtype=5), 2),
     (dict(dtype=16), 2), (dict(dtype=-1), 2),
 ])
@@ -74,6 +76,8 @@ def test_null_sessions_are_refused():
     assert L.welvet_kv_advance_device(None, 1, 16, None, None, 1, 0, None).code == 1
     assert L.welvet_kv_get_buffers(None, None).code == 1
     L.welvet_kv_release(None)
+    assert L.welvet_mha_prefill_device(None, None, r, 1, 16, 16, 16, None).code == 1
+    assert L.welvet_mha_decode_device(None, None, r, 16, 16, 16, None).code == 1
 
 
 @pytest.mark.parametrize("length,tail,cap,want", [

@@ -767,6 +767,12 @@ welvet_status welvet_kv_mount(int32_t dtype, int32_t num_pages, int32_t page_tok
   if (head_dim > wv::kKvMaxHd)
     return to_c(Status::err(wv::kUnsupported, "kv: head_dim above 256"));
   if ((int64_t)max_pages * page_tokens > (1 << 30)) return invalid("kv: capacity above 2^30");
+  // (the rows of the pool and the scores of the running sums, counted so that
+  // no product of their sizes leaves 64 bits)
+  constexpr double kMost = 1e13;
+  if ((double)num_pages * page_tokens * num_kv_heads > kMost ||
+      ((flags & WELVET_KV_TRACK) && (double)max_seqs * max_pages * page_tokens * num_heads > kMost))
+    return invalid("kv: too many pages, heads or sequences");
   if (max_seqs > 65535 || num_heads > 65535) return invalid("kv: more than 65535 sequences or heads");
   return guarded([&]() -> Status {
     WV_TRY(wv::init_device());

@@ -431,6 +431,8 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   KvPlace place;
   if (!kv_place<KT, RUNS>(p, s, a, part, lane, place)) return;
   constexpr int STRIDE = HDP + 4;
+  // one after the other: the queries' rows (16 rows of STRIDE floats), their
+  // terms (F32: none, the rows stay), the waves' sums (a multiple of the rows)
   constexpr int QBYTES = DT == kKvF32 ? 0 : T::KS * 3 * 1024, SBYTES = W * 16 * STRIDE * 4;
   __shared__ __attribute__((aligned(16))) uint8_t lds[QBYTES > SBYTES ? QBYTES : SBYTES];
   __shared__ float ml[W][16][2];
@@ -509,7 +511,7 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   const bool col_ok = c < cols;
   const float slope =
       GEN && a.alibi ? (float)(exp2(-8.0 * (double)(head0 + c + 1) / (double)p.heads) * kLog2e) : 0.0f;
-  float* qrows = reinterpret_cast<float*>(lds + QBYTES);
+  float* qrows = reinterpret_cast<float*>(lds);
   const float* q0 = a.q + (int64_t)b * a.q_stride + (int64_t)head0 * p.hd;
 #pragma unroll
   for (int r = 0; r < (16 * HDP / 4 + 64 * W - 1) / (64 * W); ++r) {
@@ -549,18 +551,26 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
     e = e < -126 || e > 126 ? 0 : e;
     mult *= pow2f(e);
     const float down = pow2f(-e);
-    for (int step = wave; step < T::KS; step += W) {
+    // this wave's steps, read before the terms take the rows' place
+    constexpr int STEPS = (T::KS + W - 1) / W;
+    v4f mine[STEPS][2];
+#pragma unroll
+    for (int r = 0; r < STEPS; ++r) {
+      const int step = wave + W * r < T::KS ? wave + W * r : 0;
+      mine[r][0] = piece(step, 0), mine[r][1] = piece(step, 1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < STEPS; ++r) {
+      const int step = wave + W * r;
+      if (step >= T::KS) break;
       bf16x8 qt[3];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const v4f x = piece(step, half);
+      for (int j = 0; j < 8; ++j) {
+        __bf16 t[3];
+        split_bf16<3>(mine[r][j / 4][j % 4] * down, t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          __bf16 t[3];
-          split_bf16<3>(x[j] * down, t);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) qt[k][4 * half + j] = t[k];
-        }
+        for (int k = 0; k < 3; ++k) qt[k][j] = t[k];
       }
 #pragma unroll
       for (int k = 0; k < 3; ++k)
@@ -574,7 +584,7 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   for (int d = 0; d < T::D; ++d) acc[d] = v4f{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.0f;
 
-  int qoff = DT == kKvF32 ? QBYTES + 4 * (c * STRIDE + 4 * g) : 16 * lane;
+  int qoff = DT == kKvF32 ? 4 * (c * STRIDE + 4 * g) : 16 * lane;
   for (int t = t0 + wave; t < t1; t += W) {
     // (the queries are read from LDS again for every tile: in registers they cost
     // a third of the waves)
