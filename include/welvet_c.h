@@ -322,7 +322,9 @@ WELVET_API welvet_status welvet_kv_read_device(welvet_kv_session* s, const welve
  * WELVET_KV_TRACK), adds to every entry's sum its weights under the
  * num_heads / num_kv_heads query heads of the K/V head. K, V or q that are
  * not finite, where they are seen, give outputs that are not finite; in
- * entries that are not seen they have no effect. */
+ * entries that are not seen they have no effect. Sums are in fp32, of weights
+ * of up to 2^8: V of up to 2^119 over the number of entries never overflows
+ * them. */
 WELVET_API welvet_status welvet_kv_attend_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,
                                                  int32_t tail, const float* q, int64_t q_stride,
                                                  double scale, int32_t window, int32_t alibi,

@@ -72,8 +72,8 @@ WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 2; 
 // Workgroups of one wave instead of four: where the sequences' rows (K/V head
 // and chunk of query heads) fill a fifth of the GPU's waves by themselves. 1000
 // sequences of 8 to 64 entries, 32 heads over 8 of 128 in bf16, 8000 rows: 79.7
-// us with four waves, 42.2 with one; 256 of 38 to 300: 57.5 and 49.4; 64 of 64
-// to 512, 16 heads of 64, 1024 rows: 29.8 and 25.2. Fewer rows with more tiles
+// us with four waves, 42.3 with one; 256 of 38 to 300: 57.5 and 48.1; 64 of 64
+// to 512, 16 heads of 64, 1024 rows: 29.8 and 24.3. Fewer rows with more tiles
 // lose: 64 x 4096 E4M3 entries, 512 rows: 77.8 and 81.7.
 WV_HD bool kv_one_wave(int64_t rows, int hd) { return rows >= 200 * kv_waves(hd); }
 
