@@ -31,4 +31,31 @@ long long kv_check_most_slots(int target) { return wv::kv_most_slots(target); }
 
 int kv_check_first_tile(int n, int qp, int window, int kt) { return wv::kv_first_tile(n, qp, window, kt); }
 
+// Walks the runs of `step` units over sequences of tiles[b] tiles as the
+// workgroups do: rows of {run, sequence, t0, t1, index, parts} in out (room for
+// `most`); returns how many there are.
+int kv_check_walk(const int* tiles, int nseq, int kt, int step, int* out, int most) {
+  const int start = wv::kKvStart / kt;
+  int rows = 0;
+  long long total = 0;
+  for (int b = 0; b < nseq; ++b) total += wv::kv_units(tiles[b], start);
+  for (long long run = 0; run * step < total; ++run) {
+    int b = 0, left = step;
+    long long off = run * step;
+    while (off >= wv::kv_units(tiles[b], start)) off -= wv::kv_units(tiles[b++], start);
+    wv::KvRun r;
+    while (wv::kv_run(tiles[b], (int)off, start, step, left, r)) {
+      if (rows == most) return -1;
+      int* o = out + 6 * rows++;
+      o[0] = (int)run, o[1] = b, o[2] = r.t0, o[3] = r.t1, o[4] = r.index, o[5] = r.parts;
+      if (left == 0 || ++b == nseq) break;
+      off = 0;
+      r = wv::KvRun();
+    }
+  }
+  return rows;
+}
+
+int kv_check_start() { return wv::kKvStart; }
+
 }  // extern "C"

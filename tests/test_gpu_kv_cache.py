@@ -212,6 +212,32 @@ def test_attend_over_many_unequal_sequences(hip, oracle, nseq, most, heads, kv, 
     c.close()
 
 
+@pytest.mark.parametrize("nseq,most,heads,kv,hd,dtype", [
+    (24, 2300, 16, 16, 64, km.BF16), (40, 1500, 32, 8, 128, km.E4M3), (33, 1200, 32, 16, 40, km.F32),
+    (12, 2100, 20, 10, 250, km.BF16), (100, 2050, 16, 8, 72, km.E4M3), (70, 2048, 16, 16, 128, km.F32),
+])
+@pytest.mark.parametrize("kind", ["plain", "track", "window"])
+def test_attend_runs_over_sequences(hip, oracle, nseq, most, heads, kv, hd, dtype, kind):
+    """Workgroups that take several sequences: empty ones between long ones, one
+    entry, whole tiles; with running sums, and windows over given positions."""
+    rng = np.random.default_rng(nseq + hd)
+    lens = rng.integers(most // 2, most + 1, nseq)
+    lens[rng.random(nseq) < 0.2] = 0
+    lens[rng.random(nseq) < 0.1] = 1
+    lens[rng.random(nseq) < 0.1] = most // 64 * 32
+    lens[nseq // 3] = most
+    c = filled(hip, oracle, lens.tolist(), dtype, heads, kv, hd, 32, seed=nseq,
+               track=kind == "track", positions=kind != "plain")
+    q = query(c.rng, c)
+    if kind == "window":
+        check(c, q, window=most // 2, alibi=True)
+    else:
+        first = check(c, q)
+        again, _ = c.attend(q)
+        assert np.array_equal(first, again)
+    c.close()
+
+
 @pytest.mark.parametrize("window,alibi,tail,scale", [
     (1, False, 0, 0.0), (17, False, 1, 0.0), (64, True, 0, 0.0), (1000, True, 1, 0.05),
     (0, True, 0, 0.0), (0, False, 1, 0.3), (2 ** 31 - 1, False, 0, 0.0), (300, False, 5, 0.0),

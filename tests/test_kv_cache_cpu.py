@@ -170,6 +170,48 @@ def test_parts_fit_the_grid_and_the_scratch(rules):
         assert rules.kv_check_parts(tiles[0], step) <= min(target, rules.kv_check_most_parts(1, target, cap))
 
 
+def test_runs_over_unequal_sequences(rules):
+    """Runs with the cost of a start: every tile in one of them, one first part
+    per sequence (also of those without tiles), the others in the runs that
+    follow it, a run's two slots never taken twice, and no more runs than target
+    and grid hold."""
+    rng = np.random.default_rng(6)
+    walked = 0
+    for _ in range(600):
+        kt = int(rng.choice([16, 32]))
+        cap = 16 * int(np.exp(rng.uniform(3, 8)))
+        nseq = int(np.exp(rng.uniform(0, 5.5))) + 1
+        lens = rng.integers(0, cap + 1, nseq) * (rng.random(nseq) < 0.8)
+        tiles = np.ascontiguousarray(-(-lens // kt), np.int32)
+        total = int(np.maximum(tiles, 1).sum())
+        target = int(rng.integers(1, 1 + max(1, total // (rules.kv_check_start() // kt))))
+        if not rules.kv_check_runs(total, target, kt):
+            continue
+        walked += 1
+        step = rules.kv_check_part_tiles(total + nseq * (rules.kv_check_start() // kt), target, kt)
+        out = np.zeros((2 * target + nseq, 6), np.int32)
+        n = rules.kv_check_walk(tiles.ctypes.data_as(ctypes.c_void_p), nseq, kt, step,
+                                out.ctypes.data_as(ctypes.c_void_p), len(out))
+        assert n >= nseq
+        out = out[:n]
+        assert out[:, 0].max() < min(target, rules.kv_check_most_parts(nseq, target, cap))
+        slots = set()
+        for b in range(nseq):
+            mine = out[out[:, 1] == b]
+            assert mine[0, 4] == 0 and np.all(mine[1:, 4] == 1) and mine[0, 5] == len(mine)
+            assert np.all(mine[:, 0] == mine[0, 0] + np.arange(len(mine)))
+            assert mine[0, 2] == 0 and mine[-1, 3] == tiles[b]
+            assert np.array_equal(mine[1:, 2], mine[:-1, 3])
+            if len(mine) > 1:
+                assert np.all(mine[:, 5] > 1) and np.all(mine[:, 3] > mine[:, 2])
+                # (as the join finds them: the first part's slot, then every second one)
+                at = 2 * mine[0, 0] + 1 + np.r_[0, 1 + 2 * np.arange(len(mine) - 1)]
+                assert np.array_equal(at, 2 * mine[:, 0] + (mine[:, 4] == 0))
+                assert not slots & set(at.tolist()) and at.max() < rules.kv_check_most_slots(target)
+                slots |= set(at.tolist())
+    assert walked > 300
+
+
 def test_first_tile_of_a_window(rules):
     for n in (0, 1, 31, 32, 33, 500):
         for window in (0, 1, 5, 32, 499, 500, 2 ** 31 - 1):

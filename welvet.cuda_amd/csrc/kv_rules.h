@@ -74,13 +74,17 @@ WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 2; 
 // sequences of 8 to 64 entries, 32 heads over 8 of 128 in bf16, 8000 rows: 79.7
 // us with four waves, 42.3 with one; 256 of 38 to 300: 57.5 and 48.1; 64 of 64
 // to 512, 16 heads of 64, 1024 rows: 29.8 and 24.3. Fewer rows with more tiles
-// lose: 64 x 4096 E4M3 entries, 512 rows: 77.8 and 81.7.
+// lose: 64 x 4096 E4M3 entries, 512 rows: 77.8 and 81.7. So do sequences that can
+// be long, kKvLong entries and more, against four waves and runs (kv_runs): 256
+// of 512 to 4096 E4M3 entries 247 us with four and 282 with one, 256 of up to
+// 2000 in bf16 221 and 248, of up to 1000 140 and 132; 1000 of up to 1100 E4M3
+// entries 474 and 307.
+constexpr int kKvLong = 2048;
 WV_HD bool kv_one_wave(int64_t rows, int hd) { return rows >= 200 * kv_waves(hd); }
 
 // Workgroups per row that fill 256 CUs once, and the tiles of `kt` entries
 // that each takes of `tiles` (one at least per sequence): two for each of four
-// waves, so that short sequences run side by side, or an equal share. Shares of
-// eight for each wave and more are runs that go over the sequences' ends.
+// waves, so that short sequences run side by side, or an equal share.
 WV_HD int kv_target(int kv_rows, int hd, bool one_wave) {
   const int n = 256 * kv_waves(hd) * (one_wave ? 4 : 1) / kv_rows;
   return n > 1 ? n : 1;
@@ -90,8 +94,36 @@ WV_HD int kv_part_tiles(int64_t tiles, int target, int kt) {
   const int64_t n = (tiles + target - 1) / target;
   return n > kKvLeastEntries / kt ? (int)n : kKvLeastEntries / kt;
 }
+// Longer shares are runs that go over the sequences' ends: 32 sequences of 512 to
+// 4096 E4M3 entries, 32 heads over 8 of 128, 25 tiles each: 37.9 us with runs,
+// 48.9 with parts; 64 of them up to 2000 40.5 and 46.1; 8 x 8192 in fp32, 16 heads
+// of 64, 52.6 and 56.6.
 WV_HD bool kv_runs(int64_t tiles, int target, int kt) {
-  return kv_part_tiles(tiles, target, kt) > 4 * (kKvLeastEntries / kt);
+  return kv_part_tiles(tiles, target, kt) > kKvLeastEntries / kt;
+}
+// Entries that a workgroup reads in the time that it takes to start another
+// sequence of its run: 64 sequences of 512 to 4096 E4M3 entries 67.9 us with 0,
+// 62.9 with 128, 61.5 with 256, 62.5 with 512.
+constexpr int kKvStart = 256;
+// A sequence in runs: `start` units and its tiles (one where it has none).
+WV_HD int kv_units(int tiles, int start) { return (tiles > 1 ? tiles : 1) + start; }
+// What a run with `left` units to go has of the sequence that it meets at unit
+// `off`: tiles [t0, t1), whether other runs have some before (index 0 or 1) and
+// how many have one; left: the units for the sequences behind. false: it ends
+// before the first tile, and the next run starts the sequence.
+struct KvRun {
+  int t0 = 0, t1 = 0, index = 0, parts = 1;
+};
+WV_HD bool kv_run(int tiles, int off, int start, int step, int& left, KvRun& r) {
+  left -= off < start ? start - off : 0;
+  if (left <= 0) return false;
+  r.t0 = off < start ? 0 : off - start;
+  const int behind = (tiles > 1 ? tiles : 1) - r.t0 - left;  // tiles for later runs
+  r.t1 = r.t0 + left < tiles ? r.t0 + left : tiles;
+  r.index = r.t0 > 0 ? 1 : 0;
+  r.parts = r.t0 > 0 ? 2 : behind > 0 ? 1 + (behind + step - 1) / step : 1;
+  left = behind < 0 ? -behind : 0;
+  return true;
 }
 WV_HD int kv_parts(int tiles, int part_tiles) {
   const int n = (tiles + part_tiles - 1) / part_tiles;

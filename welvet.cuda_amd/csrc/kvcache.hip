@@ -293,29 +293,25 @@ __device__ __forceinline__ int wave_sum(int x) {
 // its sums (KvInfo). Three ways to cut:
 //   target 0: every sequence is one part;
 //   parts of `step` tiles of one sequence each;
-//   RUNS, many tiles: runs of `step` tiles over all sequences one after the
+//   RUNS, many tiles: runs of `step` units over all sequences one after the
 //   other, the same for every workgroup however unequal the sequences are (64
 //   sequences of 512 to 4096 E4M3 entries, 32 heads over 8 of 128: parts 81.7
-//   us, runs 77.0). A workgroup then ends one sequence, may take whole ones
-//   (left: its tiles still to come) and starts another: two slots each. Few
-//   tiles are better off with parts, which a workgroup is sooner done with (16
-//   sequences of up to 8191, 12 heads over 4 of 64 with running sums: parts
-//   25.8 us, runs 29.4).
+//   us, runs 77.0). Units are tiles and what starting a sequence costs
+//   (kv_units). A workgroup ends one sequence, may take whole
+//   ones (left: its units still to come) and starts another: two slots each.
 struct KvPlace {
   int b, n, qp, t0, t1, index, parts, slot, stride, left, step;
 };
 
-// The tiles of a run that starts at tile `off` of sequence w.b.
-__device__ __forceinline__ void kv_run(int first, int tiles, int off, KvPlace& w) {
-  const int units = tiles > 1 ? tiles : 1;  // (one for a sequence without tiles)
-  w.t0 = first + off;
-  w.t1 = units - off < w.left ? first + tiles : w.t0 + w.left;
-  if (w.t1 > first + tiles) w.t1 = first + tiles;
-  w.index = off > 0 ? 1 : 0;
-  const int behind = units - off - w.left;  // tiles of the sequence for later workgroups
-  w.parts = off > 0 ? 2 : behind > 0 ? 1 + (behind + w.step - 1) / w.step : 1;
-  w.slot = 2 * (int)blockIdx.x + (off > 0 ? 0 : 1);
-  w.left = behind < 0 ? -behind : 0;
+// What a run has of sequence w.b from unit `off` on; false: none of its tiles.
+template <int KT>
+__device__ __forceinline__ bool kv_run_place(int first, int tiles, int off, KvPlace& w) {
+  KvRun r;
+  const bool has = kv_run(tiles, off, kKvStart / KT, w.step, w.left, r);
+  w.t0 = first + r.t0, w.t1 = first + r.t1;
+  w.index = r.index, w.parts = r.parts;
+  w.slot = 2 * (int)blockIdx.x + (r.index > 0 ? 0 : 1);
+  return has;
 }
 
 template <int KT, bool RUNS>
@@ -342,8 +338,9 @@ __device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const
       const int units = in ? (t > 1 ? t : 1) : 0;
       total += wave_sum(units & 0xFFFF) + ((int64_t)wave_sum(units >> 16) << 16);
     }
-    w.step = kv_part_tiles(total, part.target, KT);
     const bool runs = RUNS && kv_runs(total, part.target, KT);
+    if (runs) total += (int64_t)s.nseq * (kKvStart / KT);
+    w.step = kv_part_tiles(total, part.target, KT);
     const int64_t start = (int64_t)blockIdx.x * w.step;
     if (runs && start >= total) return false;
     int64_t units_before = 0;
@@ -353,7 +350,7 @@ __device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const
       const bool in = b0 + lane < s.nseq;
       if (s.nseq > 64 && in) kv_sequence<KT>(p, s, a, b0 + lane, n, qp, f, t);
       if (runs) {
-        const int units = in ? (t > 1 ? t : 1) : 0;
+        const int units = in ? kv_units(t, kKvStart / KT) : 0;
         const int64_t up = wave_scan(units & 0xFFFF) + ((int64_t)wave_scan(units >> 16) << 16);
         const int64_t at = start - units_before;
         hit = __ballot(in && at >= up - units && at < up);
@@ -391,8 +388,7 @@ __device__ __forceinline__ bool kv_place(const KvPool& p, const KvSeqs& s, const
     if (!hit) return false;
     if (runs) {
       w.left = w.step, w.stride = 2;
-      kv_run(first, tiles, index, w);
-      return true;
+      return kv_run_place<KT>(first, tiles, index, w);
     }
   }
   w.index = index;
@@ -408,8 +404,7 @@ __device__ __forceinline__ bool kv_next(const KvPool& p, const KvSeqs& s, const 
   ++w.b;
   int first, tiles;
   kv_sequence<KT>(p, s, a, w.b, w.n, w.qp, first, tiles);
-  kv_run(first, tiles, 0, w);
-  return true;
+  return kv_run_place<KT>(first, tiles, 0, w);
 }
 
 // GEN: ALiBi, windows, or scores for the running sums. RUNS: workgroups may take
@@ -1484,12 +1479,12 @@ Status launch_kv_read(const KvPool& p, const KvSeqs& s, int count, const int32_t
 }
 
 template <int DT>
-Status launch_attend(int hd, bool one, bool runs, dim3 grid, const KvPool& p, const KvSeqs& s, const KvAttend& a,
-                     const KvPart& part, hipStream_t st) {
-  const bool gen = a.alibi || a.window > 0 || part.scores;
+Status launch_attend(int hd, bool one, bool gen, bool runs, dim3 grid, const KvPool& p, const KvSeqs& s,
+                     const KvAttend& a, const KvPart& part, hipStream_t st) {
 #define WV_KV_HD(N)                                                                     \
   (one && gen ? k_kv_attend<DT, N, true, false, 1><<<grid, 64, 0, st>>>(p, s, a, part)    \
    : one      ? k_kv_attend<DT, N, false, false, 1><<<grid, 64, 0, st>>>(p, s, a, part)   \
+   : gen && runs ? k_kv_attend<DT, N, true, true, 4><<<grid, 256, 0, st>>>(p, s, a, part)    \
    : gen      ? k_kv_attend<DT, N, true, false, 4><<<grid, 256, 0, st>>>(p, s, a, part)   \
    : runs     ? k_kv_attend<DT, N, false, true, 4><<<grid, 256, 0, st>>>(p, s, a, part)   \
               : k_kv_attend<DT, N, false, false, 4><<<grid, 256, 0, st>>>(p, s, a, part))
@@ -1515,7 +1510,17 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   const KvPool& p = c.pool;
   const int rows = p.kv_heads * kv_chunks(p.heads / p.kv_heads);
   KvPart part;
-  const bool one = kv_one_wave((int64_t)s.nseq * rows, p.hd);
+  const bool gen = a.alibi || a.window > 0 || s.weight;
+  // (with every sequence as long as it can be)
+  const int kt = p.dtype == kKvF32 ? 16 : 32;
+  const int64_t most_tiles = (int64_t)s.nseq * ((p.capacity() + kt - 1) / kt);
+  const bool many = kv_one_wave((int64_t)s.nseq * rows, p.hd);
+  // (the general kernels need more before runs pay for their longer prologue: 16 x
+  // 8191 entries with running sums, 12 heads over 4 of 64, 26.2 us with runs, 25.5
+  // with parts, 16 x 8192 of up to 3000 20.9 and 19.1; 32 x 8192 38.2 and 41.1)
+  const bool runs = s.nseq > 1 && (!many || p.capacity() >= kKvLong) &&
+                    kv_runs(gen ? most_tiles / 2 : most_tiles, kv_target(rows, p.hd, false), kt);
+  const bool one = many && !runs;
   part.target = kv_target(rows, p.hd, one);
   int64_t parts = kv_most_parts(s.nseq, part.target, p.capacity());
   if (parts <= s.nseq) part.target = 0, parts = s.nseq;
@@ -1530,13 +1535,9 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
     part.lse2 = c.lse2.as<float>();
   }
   const dim3 grid((unsigned)parts, (unsigned)rows);
-  // (with every sequence as long as it can be)
-  const int kt = p.dtype == kKvF32 ? 16 : 32;
-  const bool runs = !one && s.nseq > 1 && part.target != 0 &&
-                    kv_runs((int64_t)s.nseq * ((p.capacity() + kt - 1) / kt), part.target, kt);
-  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, one, runs, grid, p, s, a, part, st)
-         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, one, runs, grid, p, s, a, part, st)
-                              : launch_attend<kKvE4M3>(p.hd, one, runs, grid, p, s, a, part, st));
+  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, one, gen, runs, grid, p, s, a, part, st)
+         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, one, gen, runs, grid, p, s, a, part, st)
+                              : launch_attend<kKvE4M3>(p.hd, one, gen, runs, grid, p, s, a, part, st));
   if (!finish) return Status::ok();
   const int most = (p.capacity() + 1023) / 1024;
   const int track = !s.weight ? 0 : most < 64 ? most : 64;
