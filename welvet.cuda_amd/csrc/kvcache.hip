@@ -847,7 +847,8 @@ __device__ __forceinline__ void join_sums(const float* ml, F&& at, int parts, in
 }
 
 // What follows the parts, for sequence blockIdx.z and K/V head blockIdx.y:
-// workgroups x < group join the parts of query head x; the others add the
+// workgroups x < group join the parts of query head x (none where every
+// sequence is one part); the others add the
 // heads' weights to the running sums, 1024 entries at a time (the scores are
 // there; a head's sum is formed again from its parts). A launch of its own, 4 to
 // 6 us, costs no more than a join by the workgroup that is done last, whose
@@ -856,6 +857,7 @@ __device__ __forceinline__ void join_sums(const float* ml, F&& at, int parts, in
 // with running sums 25.3 and 27.7.
 __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
   const int group = p.heads / p.kv_heads, chunks = kv_chunks(group);
+  const int joins = part.target != 0 ? group : 0;
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3;
   const size_t rows = (size_t)p.kv_heads * chunks;
@@ -866,7 +868,7 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
     const size_t slot = (size_t)info.slot + (i ? 1 + (size_t)(i - 1) * info.stride : 0);
     return (slot * rows + (size_t)h * chunks + j / 16) * most + j % 16;
   };
-  if ((int)blockIdx.x < group) {
+  if ((int)blockIdx.x < joins) {
     if (parts == 1) return;  // written by the attention itself
     const int j = blockIdx.x;
     const size_t head = (size_t)b * p.heads + (size_t)h * group + j;
@@ -914,13 +916,13 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
   }
   int n, qp, first, tiles;
   kv_sequence<16>(p, s, a, b, n, qp, first, tiles);
-  const int cap = p.capacity(), e0 = 16 * first + 1024 * ((int)blockIdx.x - group);
+  const int cap = p.capacity(), e0 = 16 * first + 1024 * ((int)blockIdx.x - joins);
   if (e0 >= n) return;
   const size_t head = (size_t)b * p.heads + (size_t)h * group;
   __shared__ float lse2[kKvFinishHeads];
   const float* sc = part.scores + head * cap;
   float* weight = s.weight + ((size_t)b * p.kv_heads + h) * cap;
-  const int step = 1024 * ((int)gridDim.x - group);
+  const int step = 1024 * ((int)gridDim.x - joins);
   for (int j0 = 0; j0 < group; j0 += kKvFinishHeads) {
     const int heads = group - j0 < kKvFinishHeads ? group - j0 : kKvFinishHeads;
     __syncthreads();
@@ -1515,15 +1517,15 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   const int kt = p.dtype == kKvF32 ? 16 : 32;
   const int64_t most_tiles = (int64_t)s.nseq * ((p.capacity() + kt - 1) / kt);
   const bool many = kv_one_wave((int64_t)s.nseq * rows, p.hd);
+  const bool whole = p.capacity() <= kv_one_part((int64_t)s.nseq * rows, many);
   // (the general kernels need more before runs pay for their longer prologue: 16 x
   // 8191 entries with running sums, 12 heads over 4 of 64, 26.2 us with runs, 25.5
   // with parts, 16 x 8192 of up to 3000 20.9 and 19.1; 32 x 8192 38.2 and 41.1)
-  const bool runs = s.nseq > 1 && (!many || p.capacity() >= kKvLong) &&
+  const bool runs = !whole && s.nseq > 1 && (!many || p.capacity() >= kKvLong) &&
                     kv_runs(gen ? most_tiles / 2 : most_tiles, kv_target(rows, p.hd, false), kt);
   const bool one = many && !runs;
-  part.target = kv_target(rows, p.hd, one);
-  int64_t parts = kv_most_parts(s.nseq, part.target, p.capacity());
-  if (parts <= s.nseq) part.target = 0, parts = s.nseq;
+  part.target = whole ? 0 : kv_target(rows, p.hd, one);
+  const int64_t parts = whole ? s.nseq : kv_most_parts(s.nseq, part.target, p.capacity());
   part.out = c.part.as<float>();
   part.ml = c.part_ml.as<float>();
   part.vec_q = p.hd % 4 == 0 && a.q_stride % 4 == 0 && (uintptr_t)a.q % 16 == 0;
@@ -1541,7 +1543,8 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   if (!finish) return Status::ok();
   const int most = (p.capacity() + 1023) / 1024;
   const int track = !s.weight ? 0 : most < 64 ? most : 64;
-  k_kv_finish<<<dim3(p.heads / p.kv_heads + track, p.kv_heads, s.nseq), 256, 0, st>>>(p, s, a, part);
+  const int joins = part.target != 0 ? p.heads / p.kv_heads : 0;
+  k_kv_finish<<<dim3(joins + track, p.kv_heads, s.nseq), 256, 0, st>>>(p, s, a, part);
   return hip_status(hipGetLastError(), "k_kv_finish");
 }
 
