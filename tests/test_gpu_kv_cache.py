@@ -455,6 +455,8 @@ def weights(rng, shape, kind):
     ([4096, 4000, 2049, 2047], 2048, 1000, 1000, True), ([16384, 9000], 9000, 4, 100, False),
     # (one workgroup's most entries; several segments, their edges, long and short rows together)
     ([32768, 20001], 16384, 4, 1000, True), ([32785, 32768, 500, 40000, 1], 1, 0, 1, False),
+    # (many rows: a workgroup each up to 32768 entries)
+    ([20000, 16385, 1, 0, 32768, 32767] + [300] * 27, 250, 4, 30, True),
     ([70001, 16384, 16385, 49152], 16384, 4, 1000, True), ([70001, 60000, 34000], 33000, 40, 20000, False),
 ])
 def test_choose(hip, lens, budget, sinks, recent, positions, kind):

@@ -960,11 +960,12 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
 // counting the digits of the keys from the top (11, 11 and 10 bits), then the
 // kept entries from behind the budget into the holes below it, both in index
 // order. Counts are whole numbers, so the order in which lanes add them does
-// not matter. Capacities of up to 32768 entries take one workgroup and one
-// launch, the keys held in registers; longer ones segments of 16384 entries
-// with a workgroup each and a launch per step (kLong, below).
+// not matter. Capacities of up to 16384 entries, with many rows 32768, take one
+// workgroup and one launch, the keys held in registers; longer ones segments of
+// 4096 entries with a workgroup each and a launch per step (k_kv_choose_long).
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
-constexpr int kChooseOne = 32 * kChooseThreads;  // most entries of one workgroup
+constexpr int kChooseLong = 16 * kChooseThreads;  // more entries may be cut into segments
+constexpr int kChooseOne = 32 * kChooseThreads;   // most entries of one workgroup
 constexpr int kDigits = 2048;
 constexpr int kShift[3] = {21, 10, 0};
 
@@ -1406,7 +1407,7 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
   WV_TRY(c->part.alloc(slots * ((hd + 3) & ~3) * sizeof(float)));
   WV_TRY(c->part_ml.alloc(slots * 2 * sizeof(float)));
   WV_TRY(c->info.alloc((size_t)max_seqs * sizeof(KvInfo)));
-  if (track && p.capacity() > kChooseOne) {
+  if (track && p.capacity() > kChooseLong) {
     const size_t choose_rows = (size_t)max_seqs * kv_heads;
     WV_TRY(c->choose_hist.alloc(choose_rows * 3 * kDigits * sizeof(uint32_t)));
     WV_HIP(hipMemsetAsync(c->choose_hist.p, 0, c->choose_hist.bytes, st));
@@ -1554,11 +1555,15 @@ Status kv_choose(const KvCache& c, const KvSeqs& s, int budget, int sinks, int r
   const KvPool& p = c.pool;
   const dim3 grid(p.kv_heads, s.nseq);
   const int cap = p.capacity();
+  // (up to kChooseOne, rows enough keep the GPU busy with a workgroup each: 8 x 20000
+  // entries of 8 heads 31.2 us so and 26.4 in segments, 32 x 20000 31.9 and 53.9; 8 x
+  // 32000 42.6 and 32.1, 32 x 32000 48.7 and 87.0)
+  const bool one = cap <= kChooseLong || (cap <= kChooseOne && (int64_t)s.nseq * p.kv_heads >= 96);
   if (cap <= 4 * kChooseThreads)
     k_kv_choose<4><<<grid, kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
-  else if (cap <= 16 * kChooseThreads)
+  else if (cap <= kChooseLong)
     k_kv_choose<16><<<grid, kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
-  else if (cap <= kChooseOne)
+  else if (one)
     k_kv_choose<32><<<grid, kChooseThreads, 0, st>>>(p, s, budget, sinks, recent, src);
   else {
     KvChooseLong l;
