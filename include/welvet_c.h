@@ -245,7 +245,8 @@ WELVET_API void welvet_mha_release(welvet_mha_session* s);
  * to nearest even) or 4 (FP8E4M3: the library's codes with one fp32 scale per
  * entry and K/V head, amax / 240 and at least 2^-96); others: code 2. A call
  * serves up to max_seqs sequences of up to capacity = max_pages * page_tokens
- * entries. The caller allots pages to sequences.
+ * entries (at most 2^30; max_seqs * capacity above 2^33 may be refused). The
+ * caller allots pages to sequences.
  *
  * Every call queues kernels on `stream` (a hipStream_t; null: the session's)
  * and returns without waiting; none allocates, so all can be captured into a

@@ -57,6 +57,16 @@ def test_mount_refusals(bad, code):
     assert not h.value
 
 
+@pytest.mark.parametrize("heads,seqs,max_pages", [(2048, 65535, 1024), (65535, 65535, 256), (1024, 40000, 1024)])
+def test_mount_refuses_more_tiles_than_a_share_can_count(heads, seqs, max_pages, rules):
+    """Shared pages allow lengths far above the pool's: a share of all sequences'
+    tiles has to stay an int."""
+    st, h = mount(pages=1, page=2 ** 20, heads=heads, kv=heads, hd=8, seqs=seqs, max_pages=max_pages)
+    assert st.code == 1 and b"capacity" in st.message and not h.value
+    tiles = seqs * (max_pages * 2 ** 20 // 16)
+    assert tiles // rules.kv_check_target(heads, 8, 0) > 2 ** 30
+
+
 def test_mount_without_a_device_is_code_2():
     if pw.lib().welvet_cuda_available():
         pytest.skip("a GPU is visible here")

@@ -296,9 +296,9 @@ __device__ __forceinline__ int wave_sum(int x) {
 //   RUNS, many tiles: runs of `step` units over all sequences one after the
 //   other, the same for every workgroup however unequal the sequences are (64
 //   sequences of 512 to 4096 E4M3 entries, 32 heads over 8 of 128: parts 81.7
-//   us, runs 77.0). Units are tiles and what starting a sequence costs
-//   (kv_units). A workgroup ends one sequence, may take whole
-//   ones (left: its units still to come) and starts another: two slots each.
+//   us, runs 77.0, and 69.0 since they count starts too: kv_units). A workgroup
+//   ends one sequence, may take whole ones (left: its units still to come) and
+//   starts another: two slots each.
 struct KvPlace {
   int b, n, qp, t0, t1, index, parts, slot, stride, left, step;
 };
