@@ -15,7 +15,12 @@ float kv_check_scale(float amax) { return wv::kv_e4m3_scale(amax); }
 
 unsigned kv_check_key(float w) { return wv::kv_weight_key(w); }
 
-int kv_check_target(int rows, int hd, int one) { return wv::kv_target(rows, hd, one != 0); }
+int kv_check_target(int rows, int hd) { return wv::kv_target(rows, hd); }
+
+// Whether one-wave workgroups have only whole sequences.
+int kv_check_one_wave(long long rows, int hd, int capacity) {
+  return wv::kv_one_wave(rows, hd, capacity) ? 1 + (capacity <= wv::kv_one_part(rows)) : 0;
+}
 
 int kv_check_runs(long long tiles, int target, int kt) { return wv::kv_runs(tiles, target, kt) ? 1 : 0; }
 

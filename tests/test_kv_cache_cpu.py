@@ -64,7 +64,7 @@ def test_mount_refuses_more_tiles_than_a_share_can_count(heads, seqs, max_pages,
     st, h = mount(pages=1, page=2 ** 20, heads=heads, kv=heads, hd=8, seqs=seqs, max_pages=max_pages)
     assert st.code == 1 and b"capacity" in st.message and not h.value
     tiles = seqs * (max_pages * 2 ** 20 // 16)
-    assert tiles // rules.kv_check_target(heads, 8, 0) > 2 ** 30
+    assert tiles // rules.kv_check_target(heads, 8) > 2 ** 30
 
 
 def test_mount_without_a_device_is_code_2():
@@ -164,7 +164,7 @@ def test_parts_fit_the_grid_and_the_scratch(rules):
             lens = np.where(rng.random(nseq) < 0.1, lens, lens // 50)
         tiles = [-(-int(n) // kt) for n in lens]
         units = [max(1, t) for t in tiles]
-        target = rules.kv_check_target(rows, int(rng.integers(1, 257)), int(rng.integers(2)))
+        target = rules.kv_check_target(rows, int(rng.integers(1, 257)))
         step = rules.kv_check_part_tiles(sum(units), target, kt)
         most, slots = rules.kv_check_most_parts(nseq, target, cap), rules.kv_check_most_slots(target)
         if rules.kv_check_runs(sum(units), target, kt):
@@ -220,6 +220,13 @@ def test_runs_over_unequal_sequences(rules):
                 assert not slots & set(at.tolist()) and at.max() < rules.kv_check_most_slots(target)
                 slots |= set(at.tolist())
     assert walked > 300
+
+
+def test_one_wave_takes_whole_sequences(rules):
+    rules.kv_check_one_wave.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
+    kinds = {rules.kv_check_one_wave(rows, hd, cap) for rows in (1, 399, 400, 600, 800, 5000, 2 ** 32)
+             for hd in (1, 64, 65, 128, 129, 256) for cap in (16, 112, 256, 1264, 2 ** 20, 2 ** 30)}
+    assert kinds == {0, 2}
 
 
 def test_first_tile_of_a_window(rules):

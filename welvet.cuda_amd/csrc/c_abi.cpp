@@ -776,7 +776,7 @@ welvet_status welvet_kv_mount(int32_t dtype, int32_t num_pages, int32_t page_tok
   if (max_seqs > 65535 || num_heads > 65535) return invalid("kv: more than 65535 sequences or heads");
   // (the attention cuts all sequences' tiles of 16 entries and more into shares,
   // which are counted as int)
-  const int shares = wv::kv_target(num_kv_heads * wv::kv_chunks(num_heads / num_kv_heads), head_dim, false);
+  const int shares = wv::kv_target(num_kv_heads * wv::kv_chunks(num_heads / num_kv_heads), head_dim);
   if ((double)max_seqs * ((double)max_pages * page_tokens / 16 + 17) / shares > (1 << 30))
     return invalid("kv: max_seqs times capacity too large");
   return guarded([&]() -> Status {

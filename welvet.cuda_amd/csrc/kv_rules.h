@@ -69,37 +69,30 @@ WV_HD int kv_chunks(int group) { return (group + 15) / 16; }
 // head dims.
 WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 2; }
 
-// Workgroups of one wave instead of four: where the sequences' rows (K/V head
-// and chunk of query heads) fill a fifth of the GPU's waves by themselves. 1000
-// sequences of 8 to 64 entries, 32 heads over 8 of 128 in bf16, 8000 rows: 79.7
-// us with four waves, 42.3 with one; 256 of 38 to 300: 57.5 and 48.1; 64 of 64
-// to 512, 16 heads of 64, 1024 rows: 29.8 and 24.3. Fewer rows with more tiles
-// lose: 64 x 4096 E4M3 entries, 512 rows: 77.8 and 81.7. So do sequences that can
-// be long, kKvLong entries and more, and are to be cut (kv_one_part), against four
-// waves and runs (kv_runs): 256 of 512 to 4096 E4M3 entries 247 us with four and
-// 282 with one, 256 of up to 2000 in bf16 221 and 248, of up to 1000 140 and 132;
-// 1000 of up to 1100 E4M3 entries 474 and 307.
-constexpr int kKvLong = 2048;
-WV_HD bool kv_one_wave(int64_t rows, int hd) { return rows >= 200 * kv_waves(hd); }
-
 // Capacity up to which every sequence is one part, so that nothing has to be
-// joined: the more rows there are, the less a cut is needed to fill the GPU.
-// Four waves, E4M3, 32 heads over 8 of 128: 1 x 400 entries 10.0 us whole and 12.1
-// cut, 4 x 800 12.7 and 12.2; 16 of up to 800 12.6 and 15.3, up to 1500 18.4 and
-// 15.6; 64 of up to 800 21.1 and 29.3, up to 2047 40.5 and 40.7. One wave, the same
-// heads: 100 of up to 800 34.5 and 33.1; 130 of up to 800 36.7 and 40.2, up to 1500
-// 61.5 and 59.6; 256 of up to 1500 99.9 and 104.7, up to 2800 200 and 176, or 69 and
-// 90 where that capacity holds 125 to 1000; 1000 of up to 300 73 and 122; 400 of up to
-// 2800 263 and 284.
-WV_HD int64_t kv_one_part(int64_t rows, bool one_wave) {
-  return one_wave ? rows * 6 / 5 - 200 : 384 + 2 * rows;
+// joined: the more rows (K/V head and chunk of query heads of every sequence)
+// there are, the less a cut is needed to fill the GPU. E4M3, 32 heads over 8 of
+// 128: 1 x 400 entries 10.0 us whole and 12.1 cut, 4 x 800 12.7 and 12.2; 16 of up
+// to 800 12.6 and 15.3, up to 1500 18.4 and 15.6; 64 of up to 800 21.1 and 29.3, up
+// to 2047 40.5 and 40.7; 256 of up to 4096 242 and 247, or 58 and 90 where that
+// capacity holds 125 to 1000.
+WV_HD int64_t kv_one_part(int64_t rows) { return 384 + 2 * rows; }
+
+// Workgroups of one wave instead of four, for many short sequences (whole ones:
+// the bound is below kv_one_part's). The same heads: 130 of up to 64 9.9 us with one
+// wave and 15.2 with four, up to 300 19.1 and 19.8, up to 800 36.9 and 32.1; 256 of
+// up to 300 28.7 and 31.0, up to 800 56.8 and 50.2; 400 of up to 800 70.0 and 73.6, up
+// to 2800 263 and 235; 1000 of up to 300 72.7 and 101.1, up to 1100 266 and 266; 256
+// fp32 ones of up to 64, 16 heads over 8 of 256, 62.1 and 79.8.
+WV_HD bool kv_one_wave(int64_t rows, int hd, int capacity) {
+  return rows >= 200 * kv_waves(hd) && capacity <= rows / 4;
 }
 
 // Workgroups per row that fill 256 CUs once, and the tiles of `kt` entries
 // that each takes of `tiles` (one at least per sequence): two for each of four
 // waves, so that short sequences run side by side, or an equal share.
-WV_HD int kv_target(int kv_rows, int hd, bool one_wave) {
-  const int n = 256 * kv_waves(hd) * (one_wave ? 4 : 1) / kv_rows;
+WV_HD int kv_target(int kv_rows, int hd) {
+  const int n = 256 * kv_waves(hd) / kv_rows;
   return n > 1 ? n : 1;
 }
 constexpr int kKvLeastEntries = 256;

@@ -408,8 +408,8 @@ __device__ __forceinline__ bool kv_next(const KvPool& p, const KvSeqs& s, const 
 }
 
 // GEN: ALiBi, windows, or scores for the running sums. RUNS: workgroups may take
-// runs over several sequences. W waves per workgroup: 4, or 1 where sequences
-// and K/V heads are many (kv_one_wave).
+// runs over several sequences. W waves per workgroup: 4, or 1 for many short
+// sequences (kv_one_wave).
 template <int DT, int HDP, bool GEN, bool RUNS, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kv_waves(HDP), 8)))
 void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
@@ -1403,7 +1403,7 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
   }
   const int chunk_rows = kv_heads * kv_chunks(heads / kv_heads);
   const int most = heads / kv_heads < 16 ? heads / kv_heads : 16;
-  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows, hd, true)) * chunk_rows * most;
+  const size_t slots = (size_t)kv_most_slots(kv_target(chunk_rows, hd)) * chunk_rows * most;
   WV_TRY(c->part.alloc(slots * ((hd + 3) & ~3) * sizeof(float)));
   WV_TRY(c->part_ml.alloc(slots * 2 * sizeof(float)));
   WV_TRY(c->info.alloc((size_t)max_seqs * sizeof(KvInfo)));
@@ -1517,15 +1517,14 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   // (with every sequence as long as it can be)
   const int kt = p.dtype == kKvF32 ? 16 : 32;
   const int64_t most_tiles = (int64_t)s.nseq * ((p.capacity() + kt - 1) / kt);
-  const bool many = kv_one_wave((int64_t)s.nseq * rows, p.hd);
-  const bool whole = p.capacity() <= kv_one_part((int64_t)s.nseq * rows, many);
+  const int target = kv_target(rows, p.hd);
+  const bool whole = p.capacity() <= kv_one_part((int64_t)s.nseq * rows);
+  const bool one = kv_one_wave((int64_t)s.nseq * rows, p.hd, p.capacity());
   // (the general kernels need more before runs pay for their longer prologue: 16 x
   // 8191 entries with running sums, 12 heads over 4 of 64, 26.2 us with runs, 25.5
   // with parts, 16 x 8192 of up to 3000 20.9 and 19.1; 32 x 8192 38.2 and 41.1)
-  const bool runs = !whole && s.nseq > 1 && (!many || p.capacity() >= kKvLong) &&
-                    kv_runs(gen ? most_tiles / 2 : most_tiles, kv_target(rows, p.hd, false), kt);
-  const bool one = many && !runs;
-  part.target = whole ? 0 : kv_target(rows, p.hd, one);
+  const bool runs = !whole && s.nseq > 1 && kv_runs(gen ? most_tiles / 2 : most_tiles, target, kt);
+  part.target = whole ? 0 : target;
   const int64_t parts = whole ? s.nseq : kv_most_parts(s.nseq, part.target, p.capacity());
   part.out = c.part.as<float>();
   part.ml = c.part_ml.as<float>();
