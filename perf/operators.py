@@ -596,7 +596,7 @@ def exact(case, seed):
                          dtype=torch.float64)
     for b, length in enumerate(_lens(case)):
         lo = max(0, length - case["window"]) if case["window"] else 0
-        back = torch.arange(length - 1, lo - 1, -1, device="cuda", dtype=torch.float64)
+        back = torch.arange(length - 1 - lo, -1, -1, device="cuda", dtype=torch.float64)
         for h in range(kv):
             K = _value64(v["k"][b, lo:length, h], case["dtype"])
             V = _value64(v["v"][b, lo:length, h], case["dtype"])
