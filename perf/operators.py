@@ -470,9 +470,9 @@ def prepare(case, seed):
 
     st["seqs"] = pw.KVSeqs(n, table.data_ptr(), v["lens"].data_ptr(), ptr("next"), ptr("pos"),
                            ptr("weight"))
+    zero = torch.zeros_like(v["lens"])
+    torch.cuda.synchronize()  # the inputs were made on another stream than the calls' own
     if kind in ("attend", "compact"):
-        torch.cuda.synchronize()  # the inputs were made on another stream
-        zero = torch.zeros_like(v["lens"])
         cache.append(pw.KVSeqs(n, table.data_ptr(), zero.data_ptr()), case["cap"],
                      v["k"].data_ptr(), v["v"].data_ptr(), v["lens"].data_ptr(), stream=st["stream"])
         torch.cuda.synchronize()
