@@ -74,3 +74,52 @@ def test_plain_forms_are_what_exact_says(cases, case, seed):
             assert np.array_equal(x.astype(np.float32), y.astype(np.float32))
         else:
             assert np.abs(x - y).max() <= 3e-5 * max(1.0, np.abs(y).max())
+
+
+class Order(OnCpu):
+    """Notes when memory is written, waited for and handed to a call."""
+
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        # (without a write: views, sizes and addresses; memory of no content)
+        if getattr(func, "__name__", "") not in ("data_ptr", "empty", "view", "__get__", "permute", "expand"):
+            self.seen.append("write")
+        return super().__torch_function__(func, types, args, kwargs)
+
+
+@pytest.mark.parametrize("case", [CASES[1], CASES[9], CASES[12], dict(
+    kind="choose", nseq=2, cap=100, ragged=True, heads=2, kv=2, budget=10, sinks=1, recent=4, moved=True)],
+    ids=lambda c: c["kind"])
+def test_calls_find_their_inputs_written(cases, case, monkeypatch):
+    """The calls run on a stream of their own: whatever they read has to be
+    waited for after its last write, by prepare() for run()."""
+    order = Order()
+
+    class Cache:
+        def __init__(self, *a):
+            pass
+
+        def append(self, *a, **kw):
+            order.seen.append("call")
+
+        attend = choose = compact = read = append
+
+    class Binding:
+        KVCache = Cache
+        KVSeqs = staticmethod(lambda *a: a)
+
+    monkeypatch.setattr(cases, "own", True)
+    monkeypatch.setattr(cases, "_stream", lambda: 1)
+    monkeypatch.setattr(cases, "_binding", lambda: Binding)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: order.seen.append("wait"))
+    with order:
+        state = cases.prepare(case, 3)
+        cases.run(state)
+    last = {"write": 0}
+    for i, what in enumerate(order.seen):
+        assert what != "call" or last.get("wait", -1) > last["write"], order.seen[max(0, i - 5):i + 1]
+        last[what] = i
+    assert "call" in last
