@@ -1053,12 +1053,14 @@ __device__ __forceinline__ int sum_before(const int* red, int wave, int lane, in
 }
 
 // The digit of the need-th key from the top of hist (every thread calls);
-// need becomes its rank among the keys of that digit.
+// need becomes its rank among the keys of that digit. (0 and 0 where hist counts
+// fewer: see KvList.)
 __device__ __forceinline__ uint32_t find_digit(const uint32_t* hist, int& need, int* red, int tid) {
   const int lane = tid & 63, wave = tid >> 6;
   const int c0 = (int)hist[kDigits - 1 - 2 * tid], c1 = (int)hist[kDigits - 2 - 2 * tid];
   const int up = wave_scan(c0 + c1);
   if (lane == 63) red[wave] = up;
+  if (tid == 0) red[kChooseWaves] = red[kChooseWaves + 1] = 0;
   __syncthreads();
   int all;
   const int before = up - c0 - c1 + sum_before(red, wave, lane, all);
@@ -1100,12 +1102,30 @@ __device__ __forceinline__ KvCounts count_cut(const KvKeys<KPT>& keys, uint32_t 
   return c;
 }
 
+// The kept entries from behind the budget: of n > budget entries, at most half
+// move. Running sums, positions or lengths that are still being written while
+// the call reads them several times can count more than there are: ranks past
+// the list are dropped on both sides, so that such a call answers nothing but
+// touches nothing outside its memory either.
+struct KvList {
+  int32_t* at;
+  uint32_t room;
+  __device__ __forceinline__ void put(int rank, int e) const {
+    if ((uint32_t)rank < room) at[rank] = e;
+  }
+  // of what place_kept left in a slot: the entry of that hole
+  __device__ __forceinline__ int take(int hole) const {
+    const uint32_t rank = (uint32_t)(-2 - hole);
+    return rank < room ? at[rank] : -1;
+  }
+};
+
 // Writes the kept entries below the budget to src, the holes' ranks in their
 // place (as -2 - rank), and the kept entries behind the budget to list. eq,
 // holes, tails: how many come before this wave.
 template <int KPT>
 __device__ __forceinline__ void place_kept(const KvKeys<KPT>& keys, const KvCut& cut, int budget,
-                                           int eq, int holes, int tails, int32_t* src, int32_t* list,
+                                           int eq, int holes, int tails, int32_t* src, const KvList& list,
                                            int lane) {
   const unsigned long long before = (1ull << lane) - 1;
   keys.each(lane, [&](int i, int e, bool in) {
@@ -1116,7 +1136,7 @@ __device__ __forceinline__ void place_kept(const KvKeys<KPT>& keys, const KvCut&
     const bool low = in && e < budget;
     const unsigned long long hs = __ballot(low && !kept), ts = __ballot(in && !low && kept);
     if (low) src[e] = kept ? e : -2 - (holes + __popcll(hs & before));
-    if (in && !low && kept) list[tails + __popcll(ts & before)] = e;
+    if (in && !low && kept) list.put(tails + __popcll(ts & before), e);
     holes += __popcll(hs);
     tails += __popcll(ts);
   });
@@ -1136,7 +1156,8 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvPool p, KvSeqs s
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   __shared__ uint32_t hist[kDigits];
   __shared__ int red[kChooseWaves + 2];
-  __shared__ int32_t list[KPT * kChooseThreads / 2];  // of n > budget entries, at most half move
+  __shared__ int32_t tail[KPT * kChooseThreads / 2];
+  const KvList list = {tail, KPT * kChooseThreads / 2};
   const int n = kv_entries(s.lens[b], 0, cap);
   int32_t* src = out + ((size_t)b * p.kv_heads + h) * budget;
   if (n <= budget) {
@@ -1167,13 +1188,13 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvPool p, KvSeqs s
   // (its own slots: every thread reads back what it wrote)
   keys.each(lane, [&](int, int e, bool) {
     const int at = e < budget ? src[e] : 0;
-    if (at < -1) src[e] = list[-2 - at];
+    if (at < -1) src[e] = list.take(at);
   });
 }
 
 // Long sequences: every step of the above a launch, a workgroup per segment of
-// kSegment entries. The digits are counted in memory (zero between calls: step
-// 4 clears them), the ranks follow from the segments' counts. 2 x 8 rows of
+// kSegment entries. The digits are counted in memory (zero between calls:
+// k_kv_fill clears them), the ranks follow from the segments' counts. 2 x 8 rows of
 // 100003 entries: 26 us in six launches of 2.5 to 7.3 us, of which each has about
 // 2 us of launch and drain (the keys are 6.4 MB, read from the caches).
 constexpr int kSegKeys = 4, kSegment = kSegKeys * kChooseThreads;
@@ -1240,10 +1261,6 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
     if (tid == 0) counts[seg] = all;
   }
   if constexpr (STEP == 4) {
-    // (the digits' counts are read no more)
-    for (int i = seg * kChooseThreads + tid; i < 3 * kDigits;
-         i += (n + kSegment - 1) / kSegment * kChooseThreads)
-      rows[i] = 0;
     // what lies in the segments before this one
     int eq0 = 0, holes0 = 0, tails0 = 0;
     for (int q0 = 0; q0 < seg; q0 += kChooseThreads) {
@@ -1271,17 +1288,21 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose_long(KvPool p, KvS
     const int low = keys.below(budget);
     const int holes = holes0 + waves_before(low - kept_low, red, wave, lane, total);
     const int tails = tails0 + waves_before(kept_high, red, wave, lane, total);
-    place_kept(keys, cut, budget, eq, holes, tails, src, c.list + (size_t)row * (cap / 2), lane);
+    const KvList list = {c.list + (size_t)row * (cap / 2), (uint32_t)cap / 2};
+    place_kept(keys, cut, budget, eq, holes, tails, src, list, lane);
   }
 }
 
-// The last step: the holes (-2 - rank) take the listed entries.
-__global__ __launch_bounds__(256) void k_kv_fill(int budget, int half, const int32_t* __restrict__ list,
-                                                 int32_t* __restrict__ out) {
+// The last step: the holes (-2 - rank) take the listed entries, and the digits'
+// counts, read no more, are cleared whatever the call found.
+__global__ __launch_bounds__(256) void k_kv_fill(int budget, int half, int32_t* __restrict__ list,
+                                                 uint32_t* __restrict__ hist, int32_t* __restrict__ out) {
   const size_t row = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
   const int j = blockIdx.x * 256 + threadIdx.x;
+  for (int i = j; i < 3 * kDigits; i += (int)gridDim.x * 256) hist[row * (3 * kDigits) + i] = 0;
+  const KvList held = {list + row * half, (uint32_t)half};
   const int at = j < budget ? out[row * budget + j] : 0;
-  if (at < -1) out[row * budget + j] = list[row * half - 2 - at];
+  if (at < -1) out[row * budget + j] = held.take(at);
 }
 
 // ---------------------------------------------------------------------------
@@ -1578,8 +1599,8 @@ Status kv_choose(const KvCache& c, const KvSeqs& s, int budget, int sinks, int r
     k_kv_choose_long<2><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
     k_kv_choose_long<3><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
     k_kv_choose_long<4><<<g, kChooseThreads, 0, st>>>(p, s, l, src);
-    k_kv_fill<<<dim3((unsigned)blocks_of(budget), p.kv_heads, s.nseq), 256, 0, st>>>(budget, cap / 2,
-                                                                                   l.list, src);
+    k_kv_fill<<<dim3((unsigned)blocks_of(budget), p.kv_heads, s.nseq), 256, 0, st>>>(
+        budget, cap / 2, l.list, l.hist, src);
   }
   return hip_status(hipGetLastError(), "k_kv_choose");
 }
