@@ -180,21 +180,26 @@ inline v2b cvt_bf16_fp8(uint32_t w, float s, bool hi) {
 // D = A B + C of 16 x 16: lane 16 q + r holds row r of A and column r of B, K
 // elements N q .. N q + N - 1, and rows 4 q + i of column r of C.
 template <int N, class T>
-v4f mfma(T a, T b, v4f c, int line) {
+v4f mfma(const T& a, const T& b, v4f c, int line) {
   const int g = give(a);
   give(b, 16);
   wave_op(line);
-  for (int i = 0; i < 4; ++i)
-    for (int q = 0; q < 4; ++q) {
-      T x, y;
-      take(g, 16 * q + 4 * (lane() / 16) + i, &x);
-      take(g, 16 * q + lane() % 16, &y, 16);
+  const auto& given = waves[cur->id >> 6].given[g];
+  const int r = lane() % 16, row = lane() / 16 * 4;
+  for (int q = 0; q < 4; ++q) {
+    T x, y;
+    memcpy(&y, given[16 * q + r] + 16, sizeof y);
+    for (int i = 0; i < 4; ++i) {
+      memcpy(&x, given[16 * q + row + i], sizeof x);
       if constexpr (N == 1) {
         c[i] += x * y;
       } else {
-        for (int k = 0; k < N; ++k) c[i] += (float)x[k] * (float)y[k];
+        typedef float vf __attribute__((ext_vector_type(N)));
+        const vf p = __builtin_convertvector(x, vf) * __builtin_convertvector(y, vf);
+        for (int k = 0; k < N; ++k) c[i] += p[k];
       }
     }
+  }
   return c;
 }
 

@@ -146,6 +146,22 @@ WV_HD int64_t kv_most_parts(int nseq, int target, int capacity) {
 // run (the end of one sequence and the start of another); without runs, there
 // are at most `target` full parts, and these sequences have one or more each.
 WV_HD int64_t kv_most_slots(int target) { return 2 * (int64_t)target; }
+// Where the sums of a sequence's parts are: part 0 in `slot`, part i > 0 in
+// slot + 1 + (i - 1) stride.
+struct KvInfo {
+  int slot, parts, stride;
+};
+// As many of these parts as there are slots for. (All of them; but where lengths
+// change during a call no workgroup may have said where a sequence's parts are,
+// and what an earlier call left there, or zeros, is found.)
+WV_HD KvInfo kv_held(KvInfo i, int slots) {
+  if (i.slot < 0 || i.slot >= slots) i.slot = 0;
+  i.stride = i.stride == 2 ? 2 : 1;
+  const int behind = slots - 1 - i.slot;
+  const int most = behind > 0 ? 2 + (behind - 1) / i.stride : 1;
+  i.parts = i.parts < 1 ? 1 : i.parts < most ? i.parts : most;
+  return i;
+}
 
 // First tile of `kt` entries that a window over indices leaves (0: no window).
 WV_HD int kv_first_tile(int n, int qp, int window, int kt) {

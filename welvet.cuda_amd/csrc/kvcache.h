@@ -73,10 +73,6 @@ struct KvAttend {
 // of a sequence of more than one), row of query heads (K/V head and chunk of
 // 16 heads) and head the reference and sum of the weights and the unscaled
 // sums of V; scores (log2 units) and lse2: for the running sums, null without.
-// Part 0 of a sequence has `slot`, part i > 0 slot + 1 + (i - 1) stride.
-struct KvInfo {
-  int slot, parts, stride;
-};
 struct KvPart {
   int target = 0;             // kv_target; 0: every sequence is one part
   bool vec_q = false, vec_out = false;  // rows of q and out hold whole 16-byte pieces

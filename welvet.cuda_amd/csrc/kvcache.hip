@@ -777,7 +777,9 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
       part.info[b] = KvInfo{place.slot, place.parts, place.stride};
     const bool one = place.parts == 1;
     const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3, quads = pitch / 4;
-    const size_t me = one ? 0 : ((size_t)place.slot * gridDim.y + blockIdx.y) * most;
+    // (lengths that change during the call can give slots past the last one)
+    const int slot = (uint32_t)place.slot < (uint32_t)kv_most_slots(part.target) ? place.slot : 0;
+    const size_t me = one ? 0 : ((size_t)slot * gridDim.y + blockIdx.y) * most;
     for (int item = threadIdx.x; item < cols * quads; item += 64 * W) {
       const int col = item / quads, quad = item - col * quads;
       float M = -INFINITY, L = 0.0f;
@@ -861,7 +863,7 @@ __global__ __launch_bounds__(256) void k_kv_finish(KvPool p, KvSeqs s, KvAttend 
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int most = group < 16 ? group : 16, pitch = (p.hd + 3) & ~3;
   const size_t rows = (size_t)p.kv_heads * chunks;
-  const KvInfo info = part.info[b];
+  const KvInfo info = kv_held(part.info[b], (int)kv_most_slots(part.target));
   const int parts = info.parts;
   // part i of head j, counted in heads
   auto of = [&](int i, int j) {
@@ -1428,6 +1430,7 @@ Status kv_build(int dtype, int num_pages, int page_tokens, int heads, int kv_hea
   WV_TRY(c->part.alloc(slots * ((hd + 3) & ~3) * sizeof(float)));
   WV_TRY(c->part_ml.alloc(slots * 2 * sizeof(float)));
   WV_TRY(c->info.alloc((size_t)max_seqs * sizeof(KvInfo)));
+  WV_HIP(hipMemsetAsync(c->info.p, 0, c->info.bytes, st));
   if (track && p.capacity() > kChooseLong) {
     const size_t choose_rows = (size_t)max_seqs * kv_heads;
     WV_TRY(c->choose_hist.alloc(choose_rows * 3 * kDigits * sizeof(uint32_t)));
