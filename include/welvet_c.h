@@ -346,7 +346,8 @@ WELVET_API welvet_status welvet_kv_choose_device(welvet_kv_session* s, const wel
                                                  int32_t* src, void* stream);
 /* Eviction, second part: entry src[..][j] moves to j wherever src is at least
  * `budget` (and within the capacity): K, V, scales, and pos and weight where
- * given. What lies behind the budget stays as it is, so the call can be
+ * given. An entry in a hole has nothing to move: slot j keeps what it holds, its
+ * pos and weight too. What lies behind the budget stays as it is, so the call can be
  * repeated. Afterwards min(lens[b], budget) entries are valid, every page
  * behind them can be given to other sequences, and K/V heads of one sequence
  * hold different tokens: pass next_pos, and pos where windows, ALiBi or

@@ -92,3 +92,12 @@ got = got[lens > 0]
 assert got.max() > 0 and got.max() - got.min() <= 2 * most * 2.0 ** -24 * got.max()
 print("done")
 """)
+
+
+@pytest.mark.parametrize("dtype", ["F32", "BF16", "E4M3"])
+def test_compact_from_a_hole(dtype):
+    clean(f"""
+import oracle_lib, test_gpu_kv_holes
+test_gpu_kv_holes.check_compact_from_a_hole(hip, oracle_lib.Oracle(), km.{dtype})
+print("done")
+""")

@@ -1324,8 +1324,9 @@ __global__ __launch_bounds__(256) void k_kv_compact(KvPool p, KvSeqs s, int budg
     const int32_t* table = s.table + (size_t)b * p.max_pages;
     from = kv_row(table, e, h, p.num_pages, p.kv_heads, p.page_tokens);
     to = kv_row(table, j, h, p.num_pages, p.kv_heads, p.page_tokens);
-    if (s.weight) s.weight[row * cap + j] = s.weight[row * cap + e];
-    if (s.pos) s.pos[row * cap + j] = s.pos[row * cap + e];
+    // (an entry in a hole has no K and V to move: the slot keeps its own whole)
+    if (s.weight && from >= 0) s.weight[row * cap + j] = s.weight[row * cap + e];
+    if (s.pos && from >= 0) s.pos[row * cap + j] = s.pos[row * cap + e];
   }
   const bool on = from >= 0 && to >= 0;
   const unsigned long long mask = __ballot(on);
