@@ -321,9 +321,12 @@ WELVET_API welvet_status welvet_kv_read_device(welvet_kv_session* s, const welve
  * [nseq][num_heads] (or null) receives the log of the sum of e^score. Without
  * any entry to see, out is 0 and lse -inf. With weight (needs
  * WELVET_KV_TRACK), adds to every entry's sum its weights under the
- * num_heads / num_kv_heads query heads of the K/V head. K, V or q that are
- * not finite, where they are seen, give outputs that are not finite; in
- * entries that are not seen they have no effect. Sums are in fp32, of weights
+ * num_heads / num_kv_heads query heads of the K/V head. In entries that are not
+ * seen nothing has an effect. In those that are, NaN in K or q, V that is not
+ * finite and scores of +inf give outputs that are not finite; an entry whose
+ * score is -inf (an infinite K against a finite q; E4M3 rows hold NaN in the
+ * place of infinities) has the weight 0, and where all are, out is 0 and lse
+ * -inf. An infinite q is not provided for. Sums are in fp32, of weights
  * of up to 2^8: V of up to 2^119 over the number of entries never overflows
  * them. */
 WELVET_API welvet_status welvet_kv_attend_device(welvet_kv_session* s, const welvet_kv_seqs* seqs,

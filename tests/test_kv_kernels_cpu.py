@@ -101,3 +101,13 @@ import oracle_lib, test_gpu_kv_holes
 test_gpu_kv_holes.check_compact_from_a_hole(hip, oracle_lib.Oracle(), km.{dtype})
 print("done")
 """)
+
+
+@pytest.mark.parametrize("dtype", ["F32", "BF16", "E4M3"])
+def test_infinite_keys(dtype):
+    clean(f"""
+import oracle_lib, test_gpu_kv_infinite
+with np.errstate(all="ignore"):
+    test_gpu_kv_infinite.check_infinite_keys(hip, oracle_lib.Oracle(), km.{dtype})
+print("done")
+""")

@@ -629,6 +629,12 @@ void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {
       }
 #pragma unroll
       for (int u = 0; u < NSUB; ++u) {
+        // (of an infinite K the query's first term has the sign; the others would
+        // make it NaN or not as their signs and zeros fall)
+        if constexpr (DT == kKvBF16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) small[u][i] = __builtin_isinf(x[u][i]) ? 0.0f : small[u][i];
+        }
         x[u] = (x[u] + small[u]) * mult;
         if constexpr (DT == kKvE4M3) x[u] *= ks[u];
       }
