@@ -107,7 +107,6 @@ print("done")
 def test_infinite_keys(dtype):
     clean(f"""
 import oracle_lib, test_gpu_kv_infinite
-with np.errstate(all="ignore"):
-    test_gpu_kv_infinite.check_infinite_keys(hip, oracle_lib.Oracle(), km.{dtype})
+test_gpu_kv_infinite.check_infinite_keys(hip, oracle_lib.Oracle(), km.{dtype})
 print("done")
 """)

@@ -142,6 +142,34 @@ WV_HD int64_t kv_most_parts(int nseq, int target, int capacity) {
   const int64_t by_capacity = (int64_t)nseq * ((capacity + kKvLeastEntries - 1) / kKvLeastEntries);
   return by_target < by_capacity ? by_target : by_capacity;
 }
+// How an attention call is cut, from what the host knows of it: sequences as
+// long as they can be, `rows` of each (K/V heads and chunks of query heads); gen:
+// ALiBi, windows or running sums. (The general kernels need more before runs pay
+// for their longer prologue: 16 x 8191 entries with running sums, 12 heads over 4
+// of 64, 26.2 us with runs, 25.5 with parts, 16 x 8192 of up to 3000 20.9 and 19.1;
+// 32 x 8192 38.2 and 41.1.)
+struct KvPlan {
+  int target;     // kv_target; 0: every sequence is one part
+  bool one, runs; // workgroups of one wave; kernels that may take runs
+  int64_t parts;  // workgroups per row
+};
+WV_HD int kv_tile(int dtype) { return dtype == kKvF32 ? 16 : 32; }
+WV_HD KvPlan kv_plan(int nseq, int rows, int hd, int capacity, int dtype, bool gen) {
+  const int kt = kv_tile(dtype), target = kv_target(rows, hd);
+  const int64_t all = (int64_t)nseq * rows, tiles = (int64_t)nseq * ((capacity + kt - 1) / kt);
+  const bool whole = capacity <= kv_one_part(all);
+  KvPlan p;
+  p.target = whole ? 0 : target;
+  p.one = kv_one_wave(all, hd, capacity);
+  p.runs = !whole && nseq > 1 && kv_runs(gen ? tiles / 2 : tiles, target, kt);
+  p.parts = whole ? nseq : kv_most_parts(nseq, target, capacity);
+  return p;
+}
+// Head dims that the attention kernel for `hd` is built for.
+WV_HD int kv_padded_hd(int dtype, int hd) {
+  if (dtype == kKvE4M3 || hd > 128) return (hd + 63) / 64 * 64;
+  return (hd + 31) / 32 * 32;
+}
 // Most slots of a row for the sums of sequences of more than one part: two per
 // run (the end of one sequence and the start of another); without runs, there
 // are at most `target` full parts, and these sequences have one or more each.

@@ -1522,19 +1522,15 @@ Status launch_attend(int hd, bool one, bool gen, bool runs, dim3 grid, const KvP
    : gen      ? k_kv_attend<DT, N, true, false, 4><<<grid, 256, 0, st>>>(p, s, a, part)   \
    : runs     ? k_kv_attend<DT, N, false, true, 4><<<grid, 256, 0, st>>>(p, s, a, part)   \
               : k_kv_attend<DT, N, false, false, 4><<<grid, 256, 0, st>>>(p, s, a, part))
-  if constexpr (DT == kKvE4M3) {
-    if (hd <= 64) WV_KV_HD(64);
-    else if (hd <= 128) WV_KV_HD(128);
-    else if (hd <= 192) WV_KV_HD(192);
-    else WV_KV_HD(256);
-  } else {
-    if (hd <= 32) WV_KV_HD(32);
-    else if (hd <= 64) WV_KV_HD(64);
-    else if (hd <= 96) WV_KV_HD(96);
-    else if (hd <= 128) WV_KV_HD(128);
-    else if (hd <= 192) WV_KV_HD(192);
-    else WV_KV_HD(256);
+  const int padded = kv_padded_hd(DT, hd);
+  if constexpr (DT != kKvE4M3) {
+    if (padded == 32) WV_KV_HD(32);
+    else if (padded == 96) WV_KV_HD(96);
   }
+  if (padded == 64) WV_KV_HD(64);
+  else if (padded == 128) WV_KV_HD(128);
+  else if (padded == 192) WV_KV_HD(192);
+  else if (padded == 256) WV_KV_HD(256);
 #undef WV_KV_HD
   return hip_status(hipGetLastError(), "k_kv_attend");
 }
@@ -1545,18 +1541,8 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
   const int rows = p.kv_heads * kv_chunks(p.heads / p.kv_heads);
   KvPart part;
   const bool gen = a.alibi || a.window > 0 || s.weight;
-  // (with every sequence as long as it can be)
-  const int kt = p.dtype == kKvF32 ? 16 : 32;
-  const int64_t most_tiles = (int64_t)s.nseq * ((p.capacity() + kt - 1) / kt);
-  const int target = kv_target(rows, p.hd);
-  const bool whole = p.capacity() <= kv_one_part((int64_t)s.nseq * rows);
-  const bool one = kv_one_wave((int64_t)s.nseq * rows, p.hd, p.capacity());
-  // (the general kernels need more before runs pay for their longer prologue: 16 x
-  // 8191 entries with running sums, 12 heads over 4 of 64, 26.2 us with runs, 25.5
-  // with parts, 16 x 8192 of up to 3000 20.9 and 19.1; 32 x 8192 38.2 and 41.1)
-  const bool runs = !whole && s.nseq > 1 && kv_runs(gen ? most_tiles / 2 : most_tiles, target, kt);
-  part.target = whole ? 0 : target;
-  const int64_t parts = whole ? s.nseq : kv_most_parts(s.nseq, part.target, p.capacity());
+  const KvPlan plan = kv_plan(s.nseq, rows, p.hd, p.capacity(), p.dtype, gen);
+  part.target = plan.target;
   part.out = c.part.as<float>();
   part.ml = c.part_ml.as<float>();
   part.vec_q = p.hd % 4 == 0 && a.q_stride % 4 == 0 && (uintptr_t)a.q % 16 == 0;
@@ -1567,10 +1553,10 @@ Status kv_attend(const KvCache& c, const KvSeqs& s, const KvAttend& a, hipStream
     part.scores = c.scores.as<float>();
     part.lse2 = c.lse2.as<float>();
   }
-  const dim3 grid((unsigned)parts, (unsigned)rows);
-  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, one, gen, runs, grid, p, s, a, part, st)
-         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, one, gen, runs, grid, p, s, a, part, st)
-                              : launch_attend<kKvE4M3>(p.hd, one, gen, runs, grid, p, s, a, part, st));
+  const dim3 grid((unsigned)plan.parts, (unsigned)rows);
+  WV_TRY(p.dtype == kKvF32    ? launch_attend<kKvF32>(p.hd, plan.one, gen, plan.runs, grid, p, s, a, part, st)
+         : p.dtype == kKvBF16 ? launch_attend<kKvBF16>(p.hd, plan.one, gen, plan.runs, grid, p, s, a, part, st)
+                              : launch_attend<kKvE4M3>(p.hd, plan.one, gen, plan.runs, grid, p, s, a, part, st));
   if (!finish) return Status::ok();
   const int most = (p.capacity() + 1023) / 1024;
   const int track = !s.weight ? 0 : most < 64 ? most : 64;
