@@ -65,3 +65,21 @@ def test_attend(hip, oracle, way, dtype, padded):
     first = check(c, q, window=max(lens) // 2)
     assert np.array_equal(first, c.attend(q, window=max(lens) // 2)[0])
     c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(km.F32, 40), (km.BF16, 64), (km.E4M3, 56)], ids=lambda x: km.NAMES.get(x, x))
+def test_runs_over_many_sequences(hip, oracle, dtype, hd):
+    """More sequences than a wave has lanes, most of them short."""
+    n, heads, kv = 70, 16, 16
+    rng = np.random.default_rng(hd)
+    lens = rng.integers(0, 600, n)
+    lens[rng.random(n) < 0.2] = 0
+    lens[[0, 40, 69]] = 1, 2990, 700
+    assert kp.kernel(n, heads, kv, hd, 3008, dtype, False)[3] and kp.takes_runs(lens, heads, kv, hd, dtype)
+    c = filled(hip, oracle, lens.tolist(), dtype, heads, kv, hd, 16, seed=hd, track=False, room=18)
+    q = query(c.rng, c)
+    first = check(c, q)
+    assert c.cap == 3008 and np.array_equal(first, c.attend(q)[0])
+    check(c, q, alibi=True)
+    c.close()

@@ -71,12 +71,27 @@ WV_HD constexpr int kv_waves(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 2; 
 
 // Capacity up to which every sequence is one part, so that nothing has to be
 // joined: the more rows (K/V head and chunk of query heads of every sequence)
-// there are, the less a cut is needed to fill the GPU. E4M3, 32 heads over 8 of
-// 128: 1 x 400 entries 10.0 us whole and 12.1 cut, 4 x 800 12.7 and 12.2; 16 of up
-// to 800 12.6 and 15.3, up to 1500 18.4 and 15.6; 64 of up to 800 21.1 and 29.3, up
-// to 2047 40.5 and 40.7; 256 of up to 4096 242 and 247, or 58 and 90 where that
-// capacity holds 125 to 1000.
-WV_HD int64_t kv_one_part(int64_t rows) { return 384 + 2 * rows; }
+// there are, the less a cut is needed to fill the GPU, and the more bytes an
+// entry's K and V have, the sooner it pays. A call's us whole and cut, of n
+// sequences of an eighth of the capacity to all of it:
+//   E4M3, 32 heads over 8 of 128 (256 bytes): 1 x 400 9.9 and 12.0, 1 x 600 10.9 and
+//     12.3, 4 x 800 12.8 and 12.4, 16 x 800 12.8 and 15.3, 16 x 1500 18.3 and 15.5,
+//     64 x 800 20.2 and 28.7, 64 x 2047 39.2 and 41.3, 256 x 4096 238 and 242
+//   bf16, the same heads (512): 1 x 400 11.0 and 13.2, 16 x 800 15.6 and 17.1, 64 x 800
+//     28.6 and 34.3, 64 x 2047 59.7 and 57.0
+//   bf16, 12 over 4 of 64 (256): 1 x 600 9.0 and 11.5, 64 x 1200 14.7 and 19.0, 256 x
+//     2400 71.2 and 67.3
+//   fp32, 16 over 8 of 256 (2048): 1 x 400 36.2 and 29.8, 16 x 400 44.7 and 37.1, 64 x 1600
+//     318 and 264, 256 x 1500 893 and 887
+// The bound stays below where both meet at many rows, as one long sequence among
+// short ones is then one workgroup's: 100 and one of 2047 among 64 34.7 whole, 20.2
+// cut; 200 and one of 4096 among 256 91.3 and 68.8; among 1000, one of 8000 182 and
+// 265, one of 16384 266 and 273. It goes by the capacity, as the host does not know
+// the lengths: 256 of 125 to 1000 in a capacity of 4096 58 whole, 90 cut.
+WV_HD int64_t kv_one_part(int64_t rows, int entry_bytes = 256) {
+  const int64_t n = (650000 + 1350 * rows) / (512 + (entry_bytes > 256 ? entry_bytes : 256));
+  return n > 256 ? n : 256;
+}
 
 // Workgroups of one wave instead of four, for many short sequences (whole ones:
 // the bound is below kv_one_part's). The same heads: 130 of up to 64 9.9 us with one
@@ -157,7 +172,7 @@ WV_HD int kv_tile(int dtype) { return dtype == kKvF32 ? 16 : 32; }
 WV_HD KvPlan kv_plan(int nseq, int rows, int hd, int capacity, int dtype, bool gen) {
   const int kt = kv_tile(dtype), target = kv_target(rows, hd);
   const int64_t all = (int64_t)nseq * rows, tiles = (int64_t)nseq * ((capacity + kt - 1) / kt);
-  const bool whole = capacity <= kv_one_part(all);
+  const bool whole = capacity <= kv_one_part(all, 2 * hd * kv_elem_bytes(dtype));
   KvPlan p;
   p.target = whole ? 0 : target;
   p.one = kv_one_wave(all, hd, capacity);
