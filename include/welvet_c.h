@@ -252,7 +252,11 @@ WELVET_API void welvet_mha_release(welvet_mha_session* s);
  * and returns without waiting; none allocates, so all can be captured into a
  * graph, and all lengths and tables are read on the device when they run.
  * Calls on one session must not overlap in time, on the device either (they
- * share the scratch); replays of graphs captured from it count as calls. */
+ * share the scratch); replays of graphs captured from it count as calls. Buffers
+ * that a call reads hold still while it runs (work of other streams that fills
+ * them is waited for first): some are read several times, and with values that
+ * change between, the results are undefined, though nothing outside the call's
+ * buffers is touched. */
 typedef struct welvet_kv_session welvet_kv_session;
 /* The sequences of a call: device buffers of the caller, 4-byte aligned, pos
  * and weight 16-byte aligned.
@@ -377,8 +381,10 @@ WELVET_API welvet_status welvet_kv_advance_device(welvet_kv_session* s, int32_t 
  * next_pos[b] (RoPE layers), K and V appended, pre [nseq*q_dim] is the
  * attention over the sequence's entries and the new one, post [nseq*d_model]
  * its O projection. The layer's window and ALiBi hold; its causal,
- * bidirectional and prefix masks all leave the whole past. lens and next_pos
- * stay as they are (welvet_kv_advance_device, once all layers have run). A
+ * bidirectional and prefix masks all leave the whole past. The layer's
+ * max_seq_len bounds a prefill's tokens (as a forward's) and is the window of a
+ * windowed layer that was given none; tokens are decoded at any position, up to
+ * the cache's capacity. lens and next_pos stay as they are (welvet_kv_advance_device, once all layers have run). A
  * sequence at its capacity keeps its entries: the token is not stored and
  * attends to them alone. */
 WELVET_API welvet_status welvet_mha_prefill_device(welvet_mha_session* m, welvet_kv_session* s,

@@ -295,10 +295,10 @@ __device__ __forceinline__ int wave_sum(int x) {
 //   parts of `step` tiles of one sequence each;
 //   RUNS, many tiles: runs of `step` units over all sequences one after the
 //   other, the same for every workgroup however unequal the sequences are (64
-//   sequences of 512 to 4096 E4M3 entries, 32 heads over 8 of 128: parts 81.7
-//   us, runs 77.0, and 69.0 since they count starts too: kv_units). A workgroup
-//   ends one sequence, may take whole ones (left: its units still to come) and
-//   starts another: two slots each.
+//   sequences of 512 to 4096 E4M3 entries, 32 heads over 8 of 128, whole calls:
+//   parts 81.7 us, runs 75.7, and 69.0 since they count starts too: kv_units). A
+//   workgroup ends one sequence, may take whole ones (left: its units still to
+//   come) and starts another: two slots each.
 struct KvPlace {
   int b, n, qp, t0, t1, index, parts, slot, stride, left, step;
 };
@@ -409,7 +409,13 @@ __device__ __forceinline__ bool kv_next(const KvPool& p, const KvSeqs& s, const 
 
 // GEN: ALiBi, windows, or scores for the running sums. RUNS: workgroups may take
 // runs over several sequences. W waves per workgroup: 4, or 1 for many short
-// sequences (kv_one_wave).
+// sequences (kv_one_wave). Some RUNS kernels keep up to 20 registers in scratch
+// (256 dims; general ones of 64 and 128) and are faster than parts all the same:
+// 32 sequences of 512 to 4096, 16 heads over 8 of 256, fp32 297 us with runs and 410
+// with parts, general 295 and 420, bf16 120 and 157, 128 and 166; 32 over 8 of 128,
+// general, bf16 58.5 and 70.2, E4M3 42.5 and 55.5; 64 of 750 to 6000, E4M3, 16 over
+// 8 of 64, 50.8 and 56.2, general 66 and 77, bf16, 12 over 4 of 64, general 45.8 and
+// 52.8.
 template <int DT, int HDP, bool GEN, bool RUNS, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(kv_waves(HDP), 8)))
 void k_kv_attend(KvPool p, KvSeqs s, KvAttend a, KvPart part) {

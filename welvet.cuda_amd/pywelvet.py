@@ -614,7 +614,10 @@ KV_TRACK = 1
 
 class KVCache:
     """A paged K/V cache (welvet_kv_*). Buffers are device pointers; every call
-    returns without waiting, on `stream` or the session's own."""
+    returns without waiting, on `stream` or the session's own: what it reads has
+    to be written by work of that stream, or waited for. `track` allots scratch
+    of max_seqs * heads * capacity floats for the running sums: pass False where
+    none are kept."""
 
     def __init__(self, dtype, num_pages, page_tokens, heads, kv_heads, head_dim, max_seqs,
                  max_pages, track=True):
