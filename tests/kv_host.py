@@ -68,7 +68,7 @@ def build(to):
         src = os.path.join(to, name + ".cpp")
         with open(src, "w") as f:
             f.write(text)
-        jobs.append(subprocess.Popen([CLANG, "-O2", "-mavx2", "-std=c++17", "-fPIC", "-w", "-I" + SIMT, "-I" + CSRC,
+        jobs.append(subprocess.Popen([CLANG, "-O2", "-std=c++17", "-fPIC", "-w", "-I" + SIMT, "-I" + CSRC,
                                       "-I" + os.path.join(ROOT, "include"), "-c", src, "-o", src + ".o"]))
     for j in jobs:
         if j.wait():

@@ -1209,7 +1209,7 @@ __global__ __launch_bounds__(kChooseThreads) void k_kv_choose(KvPool p, KvSeqs s
 // Long sequences: every step of the above a launch, a workgroup per segment of
 // kSegment entries. The digits are counted in memory (zero between calls:
 // k_kv_fill clears them), the ranks follow from the segments' counts. 2 x 8 rows of
-// 100003 entries: 26 us in six launches of 2.5 to 7.3 us, of which each has about
+// 100003 entries: 26 us in six launches of 2.0 to 7.0 us, of which each has about
 // 2 us of launch and drain (the keys are 6.4 MB, read from the caches).
 constexpr int kSegKeys = 4, kSegment = kSegKeys * kChooseThreads;
 
