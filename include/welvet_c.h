@@ -354,8 +354,8 @@ WELVET_API welvet_status welvet_kv_choose_device(welvet_kv_session* s, const wel
 /* Eviction, second part: entry src[..][j] moves to j wherever src is at least
  * `budget` (and within the capacity): K, V, scales, and pos and weight where
  * given. An entry in a hole has nothing to move: slot j keeps what it holds, its
- * pos and weight too. What lies behind the budget stays as it is, so the call can be
- * repeated. Afterwards min(lens[b], budget) entries are valid, every page
+ * pos and weight too. What lies behind the budget stays as it is, so the call
+ * can be repeated. Afterwards min(lens[b], budget) entries are valid, every page
  * behind them can be given to other sequences, and K/V heads of one sequence
  * hold different tokens: pass next_pos, and pos where windows, ALiBi or
  * further eviction need positions. Pages that sequences share are not for
@@ -384,9 +384,10 @@ WELVET_API welvet_status welvet_kv_advance_device(welvet_kv_session* s, int32_t 
  * bidirectional and prefix masks all leave the whole past. The layer's
  * max_seq_len bounds a prefill's tokens (as a forward's) and is the window of a
  * windowed layer that was given none; tokens are decoded at any position, up to
- * the cache's capacity. lens and next_pos stay as they are (welvet_kv_advance_device, once all layers have run). A
- * sequence at its capacity keeps its entries: the token is not stored and
- * attends to them alone. */
+ * the cache's capacity. lens and next_pos stay as they are
+ * (welvet_kv_advance_device, once all layers have run). A sequence at its
+ * capacity keeps its entries: the token is not stored and attends to them
+ * alone. */
 WELVET_API welvet_status welvet_mha_prefill_device(welvet_mha_session* m, welvet_kv_session* s,
                                                    const welvet_kv_seqs* seqs, int32_t tokens,
                                                    const float* x, float* pre, float* post,
